@@ -289,6 +289,194 @@ int zwg_kv_append_batch(zwg_kv *kv, uint64_t layer, uint64_t seq0, uint64_t n_se
 int zwg_kv_read(zwg_kv *kv, uint64_t layer, uint64_t seq, float *k_host, float *v_host);
 
 /*
+ * Rotary positions as an operator of their own: the rotation of src/llm.zig:221-238 (which the caches
+ * above apply inside their append, in its one form) over any rows of heads, in both pair layouts, over
+ * part of a head, and with frequencies scaled for contexts longer than the trained one.
+ *
+ * Pair j < n_rot/2 of a head is (x_j, x_{j + n_rot/2}) in ZWG_ROPE_HALF (as src/llm.zig:221-238), and
+ * (x_2j, x_{2j+1}) in ZWG_ROPE_INTERLEAVED; dims from n_rot on stay as they are.  At position p
+ *     y_a = x_a c - x_b s,   y_b = x_a s + x_b c,   c = f32(m cos(p w_j)), s = f32(m sin(p w_j)),
+ * each product and sum rounded to f32, the angles in f64.  With w = base^(-2j / n_rot), f = factor:
+ *   ZWG_ROPE_NONE    w_j = w                               (factor must be 1)
+ *   ZWG_ROPE_LINEAR  w_j = w / f                           (positions interpolated)
+ *   ZWG_ROPE_NTK     w_j of base * f^(n_rot / (n_rot - 2)) (the slowest pair slowed by f, the fastest kept)
+ *   ZWG_ROPE_YARN    w_j = g w + (1 - g) w / f, g = clamp((n_orig w / 2 pi - beta_slow) / (beta_fast -
+ *                    beta_slow), 0, 1): pairs that turn often over the n_orig trained positions stay
+ * m is mscale; 0 takes 0.1 ln(f) + 1 for YARN with f > 1, and 1 otherwise.
+ */
+typedef struct zwg_rope zwg_rope;
+
+#define ZWG_ROPE_HALF 0u
+#define ZWG_ROPE_INTERLEAVED 1u
+
+#define ZWG_ROPE_NONE 0u
+#define ZWG_ROPE_LINEAR 1u
+#define ZWG_ROPE_NTK 2u
+#define ZWG_ROPE_YARN 3u
+
+typedef struct zwg_rope_desc {
+    uint64_t n_ctx;     /* positions 0 .. n_ctx - 1, below 2^31 / n_rot */
+    uint64_t d;         /* head dim, a multiple of 4 up to 1024 */
+    uint64_t n_rot;     /* rotated dims, even, 2 .. d (NTK: 4 .. d) */
+    uint32_t layout;    /* ZWG_ROPE_HALF or ZWG_ROPE_INTERLEAVED */
+    uint32_t scaling;   /* ZWG_ROPE_NONE .. ZWG_ROPE_YARN */
+    double base;        /* > 0 */
+    double factor;      /* >= 1 */
+    uint64_t n_orig;    /* YARN: the trained positions, >= 1 */
+    double beta_fast;   /* YARN: turns above which a pair stays (0: 32) */
+    double beta_slow;   /* YARN: turns below which a pair slows by factor (0: 1) */
+    double mscale;      /* factor on cos and sin; 0: the method's own */
+} zwg_rope_desc;
+
+/* Flag of zwg_rope_apply_dev: rotate by the negative angle (y = m R^T x): the backward pass of the
+ * rotation, and, with m = 1, its inverse. */
+#define ZWG_ROPE_INVERSE 1u
+
+/* Build the tables on ctx's device (two of n_ctx * n_rot / 2 floats; waits for the device).  *out is NULL on
+ * failure.  zwg_close of the context frees the tables of a zwg_rope not destroyed yet, which then only
+ * accepts zwg_rope_destroy; a zwg_kvq made with it keeps the tables it needs. */
+int zwg_rope_create(zwg_ctx *ctx, const zwg_rope_desc *desc, zwg_rope **out);
+void zwg_rope_destroy(zwg_rope *rope);
+
+/*
+ * out rows = the rotated x rows: n tokens, n_head heads of d each, token i's row at x + i*x_stride
+ * and out + i*out_stride (floats, multiples of 4, at least n_head*d).  out may be x with the same stride (in
+ * place); otherwise the two must not overlap.  Token i is at position pos_dev[i] (device int32[n]) or, with
+ * pos_dev NULL, pos0 + i.  A position of pos_dev outside [0, n_ctx) skips its row: nothing of it is written.
+ * Only the n_head*d columns of a row are written.  Device pointers, 16-byte aligned, asynchronous on the
+ * context's stream.
+ */
+int zwg_rope_apply_dev(zwg_rope *rope, const float *x, uint64_t n, uint64_t n_head, uint64_t x_stride,
+                       const int32_t *pos_dev, uint64_t pos0, float *out, uint64_t out_stride, uint32_t flags);
+
+/*
+ * Key/value caches held in 8 bits: what zwg_kv is, at a quarter of the bytes, for long contexts.  Per
+ * (layer, sequence, KV head) the tokens form blocks of `block`, and the keys of a block share one f32
+ * scale, its values another.  The contents are defined bit for bit: with amax the largest magnitude in
+ * the block's rows (after rotation) and Q = 127 (ZWG_KVQ_I8) or 448 (ZWG_KVQ_E4M3),
+ *     scale = f32(amax / Q),  code = round(f32(x * f32(Q / amax))) to the nearest code, ties to even,
+ * and an element stands for f32(code * scale).  A block with amax below 2^-100 holds zeros.  A block with an
+ * infinity or a NaN in it reads as NaN throughout (never as wrong finite values).
+ *
+ * An append of n rows at position pos ends its sequence at pos + n: the rows of the block of position
+ * pos + n - 1 behind it become zeros; blocks after it keep what they held.  A block being filled also
+ * keeps its rows in f32, so its contents are those of its rows whatever calls brought them; rows of
+ * a block reopened later (an append into a block that is not the one last appended to) count as
+ * the values they stand for.
+ */
+typedef struct zwg_kvq zwg_kvq;
+
+#define ZWG_KVQ_I8 0u   /* whole numbers -127 .. 127 */
+#define ZWG_KVQ_E4M3 1u /* 8-bit floating point, 4 exponent and 3 mantissa bits, no infinities, up to 448 */
+
+typedef struct zwg_kvq_desc {
+    uint64_t n_layer;
+    uint64_t n_seq;
+    uint64_t n_ctx;     /* positions per sequence; n_ctx * d below 2^31 - 2^20 */
+    uint64_t n_head_kv;
+    uint64_t d;         /* 32, 64 or 128 */
+    uint64_t block;     /* tokens per scale: 16, 32 or 64 */
+    uint32_t format;    /* ZWG_KVQ_I8 or ZWG_KVQ_E4M3 */
+    uint32_t reserved;  /* must be 0 */
+} zwg_kvq_desc;
+
+/* Allocate the caches (all zeros).  rope (may be NULL, else of the same context and head dim) rotates the
+ * appended keys, and q.  Lifetimes as zwg_kv's. */
+int zwg_kvq_create(zwg_ctx *ctx, const zwg_kvq_desc *desc, const zwg_rope *rope, zwg_kvq **out);
+void zwg_kvq_destroy(zwg_kvq *kv);
+/* Device bytes that the caches of `desc` take (codes, scales and the open blocks), without any rotary tables; 0
+ * for a desc that zwg_kvq_create refuses.  Host-only. */
+uint64_t zwg_kvq_bytes(const zwg_kvq_desc *desc);
+
+/*
+ * Append n rows to (layer, seq) at positions pos .. pos+n-1 (pos + n <= n_ctx): k_rows, v_rows
+ * [n][n_head_kv*d] device f32, 16-byte aligned.  With a rope the keys are rotated at rotary positions rope_pos ..
+ * rope_pos+n-1 (which differ from pos once tokens have been evicted), and so is q, if not NULL: q
+ * rows of q_stride floats (n_head heads of d) to q_out rows of q_stride (q_out may be q).  Without a
+ * rope, rope_pos is ignored and q must be NULL.  Asynchronous on the context's stream.
+ */
+int zwg_kvq_append(zwg_kvq *kv, uint64_t layer, uint64_t seq, uint64_t pos, uint64_t n, uint64_t rope_pos,
+                   const float *k_rows, const float *v_rows, const float *q, float *q_out, uint64_t n_head,
+                   uint64_t q_stride);
+
+/* One new row for each of the sequences seq0 .. seq0+n_seq-1 at the positions in the device int32 array
+ * pos_dev[n_seq], rotated at rope_pos_dev[n_seq] (NULL: pos_dev).  A sequence whose position (or, with a
+ * rope, whose rotary position) is outside the cache (the tables) is skipped: neither its cache nor its q_out
+ * row is written. */
+int zwg_kvq_append_batch(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const int32_t *pos_dev,
+                         const int32_t *rope_pos_dev, const float *k_rows, const float *v_rows, const float *q,
+                         float *q_out, uint64_t n_head, uint64_t q_stride);
+
+/* The values that n positions stand for, of layers layer0 .. layer0+n_layer-1 and sequences seq0 ..
+ * seq0+n_seq-1: k_out, v_out (either may be NULL) [n_layer][n_seq][n][n_head_kv*d] device f32, 16-byte aligned.
+ * Sequence i's positions begin at pos_dev[i] (device int32[n_seq]) or, with pos_dev NULL, at pos0;
+ * elements of positions outside [0, n_ctx) are not written.  Asynchronous. */
+int zwg_kvq_rows_dev(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq,
+                     const int32_t *pos_dev, uint64_t pos0, uint64_t n, float *k_out, float *v_out);
+
+/*
+ * Attention over the caches: for each of the n_seq sequences from seq0, n_q queries attend to its first n_kv
+ * keys, as zwg_attention_batch_dev does over f32 caches (src/ops.zig:464-605): query head h reads KV
+ * head h / (n_head / n_head_kv), scores are scaled by f32(1/sqrt(d)), and causal query i sees keys
+ * j <= n_kv - n_q + i.  A query that sees no key gives zeros.  The products are f16 MFMA over the codes (exact in
+ * f16) and over queries and probabilities split into f16 hi + lo terms, scaled to f16's range row by row, with
+ * f32 accumulation: f32-level accuracy for any finite input, measured at most 3e-7 normwise relative beyond what
+ * the scores' own f32 rounding gives.
+ *
+ * weights (may be NULL): device f32, sequence i's at weights + i*weights_bstride, KV head h's row at
+ * h*weights_stride (at least n_kv; floats).  The row's first n_kv elements become decay * old + the sum
+ * over the call's queries and over the heads that share the KV head of each key's probability (decay 0: the old
+ * values are not read); later elements are left alone.  Sums are taken in a fixed order.
+ */
+typedef struct zwg_kvq_attn {
+    uint64_t n_q;
+    uint64_t n_kv;            /* keys, or with n_kv_dev the most that any sequence has; at most n_ctx */
+    uint64_t n_head;
+    uint64_t q_stride;        /* floats between queries; multiples of 4, at least n_head * d */
+    uint64_t out_stride;
+    uint64_t q_bstride;       /* floats between sequences; multiples of 4 */
+    uint64_t out_bstride;
+    uint64_t weights_stride;  /* with weights */
+    uint64_t weights_bstride;
+    const int32_t *n_kv_dev;  /* device int32[n_seq], each sequence's keys (clamped to 0 .. n_kv), or NULL */
+    float decay;              /* with weights: finite, >= 0 */
+    uint32_t causal;
+} zwg_kvq_attn;
+
+int zwg_kvq_attention_dev(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const float *q,
+                          const zwg_kvq_attn *attn, float *out, float *weights);
+
+/*
+ * Eviction by accumulated weight: cut sequences seq0 .. seq0+n_seq-1 of layers layer0 .. layer0+n_layer-1
+ * to n_keep tokens each.  Per (layer, sequence, KV head) with n_kv > n_keep tokens: the first
+ * n_first, the last n_recent and, of those between, the n_keep - n_first - n_recent of the largest weights
+ * stay (equal weights: the lower position; a NaN counts as larger than any number), move to positions
+ * 0 .. n_keep-1 in their order, and form new blocks: the values that they stand for, quantised as an append
+ * quantises (keys keep the rotation of the position they were appended at).  Rows behind n_keep in the last
+ * block become zeros.  Heads of one sequence keep tokens of their own.  Sequences of at most n_keep tokens are
+ * left as they are.
+ *
+ * weights, weights_out: device f32, (layer l, sequence i, head h)'s row at ((l * n_seq + i) * n_head_kv + h) *
+ * weights_stride, counted from layer0 and seq0.  weights_out (may be weights, or NULL) gets the kept tokens' weights
+ * at their new positions and zeros from there up to n_kv (the most that any sequence has).  kept (may be NULL):
+ * int32 [n_layer][n_seq][n_head_kv][n_keep], the old positions of the kept tokens, -1 past
+ * a shorter sequence's end.  n_kv_out (may be n_kv_dev, or NULL): int32[n_seq], min(n_kv, n_keep).
+ */
+typedef struct zwg_kvq_cut {
+    uint64_t n_kv;            /* tokens, or with n_kv_dev the most that any sequence has; at most n_ctx */
+    uint64_t n_keep;          /* >= 1 */
+    uint64_t n_first;         /* n_first + n_recent <= n_keep */
+    uint64_t n_recent;
+    uint64_t weights_stride;  /* at least n_kv */
+    const int32_t *n_kv_dev;  /* device int32[n_seq] (clamped to 0 .. n_kv), or NULL */
+    int32_t *n_kv_out;
+    int32_t *kept;
+} zwg_kvq_cut;
+
+int zwg_kvq_evict_dev(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq,
+                      const zwg_kvq_cut *cut, const float *weights, float *weights_out);
+
+/*
  * Linear layers: the drop-in for ops.linear (src/ops.zig:283-306) with f16 weights, the encoder's
  * Q/K/V/O projections and MLP (src/encoder.zig:164-174), BERT's (src/bert.zig:223-232) and the
  * scene model's (src/scene.zig:369-378).  out[i][o] = sum_p x[i][p] * w[o][p] (+ bias[o]), with

@@ -265,6 +265,94 @@ pub extern "zwgpu" fn zwg_llm_forward_scratch(n: u64, n_embd: u64, n_ff: u64) u6
 pub extern "zwgpu" fn zwg_llm_forward_dev(ctx: *Ctx, lm: *const Llm, tokens: [*]const i32, n: u64, seq: u64,
     pos0: u64, logits: [*]f32, scratch: [*]f32) c_int;
 
+// ---- rotary positions (zw_gpu.h: zwg_rope_*)
+
+pub const Rope = opaque {};
+pub const ROPE_HALF: u32 = 0;
+pub const ROPE_INTERLEAVED: u32 = 1;
+pub const ROPE_NONE: u32 = 0;
+pub const ROPE_LINEAR: u32 = 1;
+pub const ROPE_NTK: u32 = 2;
+pub const ROPE_YARN: u32 = 3;
+pub const ROPE_INVERSE: u32 = 1;
+
+pub const RopeDesc = extern struct {
+    n_ctx: u64,
+    d: u64,
+    n_rot: u64,
+    layout: u32 = ROPE_HALF,
+    scaling: u32 = ROPE_NONE,
+    base: f64,
+    factor: f64 = 1,
+    n_orig: u64 = 0,
+    beta_fast: f64 = 0,
+    beta_slow: f64 = 0,
+    mscale: f64 = 0,
+};
+
+pub extern "zwgpu" fn zwg_rope_create(ctx: *Ctx, desc: *const RopeDesc, out: *?*Rope) c_int;
+pub extern "zwgpu" fn zwg_rope_destroy(rope: ?*Rope) void;
+pub extern "zwgpu" fn zwg_rope_apply_dev(rope: *Rope, x: [*]const f32, n: u64, n_head: u64, x_stride: u64,
+    pos_dev: ?[*]const i32, pos0: u64, out: [*]f32, out_stride: u64, flags: u32) c_int;
+
+// ---- key/value caches in 8 bits (zw_gpu.h: zwg_kvq_*)
+
+pub const Kvq = opaque {};
+pub const KVQ_I8: u32 = 0;
+pub const KVQ_E4M3: u32 = 1;
+
+pub const KvqDesc = extern struct {
+    n_layer: u64,
+    n_seq: u64,
+    n_ctx: u64,
+    n_head_kv: u64,
+    d: u64,
+    block: u64,
+    format: u32 = KVQ_I8,
+    reserved: u32 = 0,
+};
+
+pub const KvqAttn = extern struct {
+    n_q: u64,
+    n_kv: u64,
+    n_head: u64,
+    q_stride: u64,
+    out_stride: u64,
+    q_bstride: u64,
+    out_bstride: u64,
+    weights_stride: u64 = 0,
+    weights_bstride: u64 = 0,
+    n_kv_dev: ?[*]const i32 = null,
+    decay: f32 = 1,
+    causal: u32,
+};
+
+pub const KvqCut = extern struct {
+    n_kv: u64,
+    n_keep: u64,
+    n_first: u64 = 0,
+    n_recent: u64 = 0,
+    weights_stride: u64,
+    n_kv_dev: ?[*]const i32 = null,
+    n_kv_out: ?[*]i32 = null,
+    kept: ?[*]i32 = null,
+};
+
+pub extern "zwgpu" fn zwg_kvq_create(ctx: *Ctx, desc: *const KvqDesc, rope: ?*const Rope, out: *?*Kvq) c_int;
+pub extern "zwgpu" fn zwg_kvq_destroy(kv: ?*Kvq) void;
+pub extern "zwgpu" fn zwg_kvq_bytes(desc: *const KvqDesc) u64;
+pub extern "zwgpu" fn zwg_kvq_append(kv: *Kvq, layer: u64, seq: u64, pos: u64, n: u64, rope_pos: u64,
+    k_rows: [*]const f32, v_rows: [*]const f32, q: ?[*]const f32, q_out: ?[*]f32, n_head: u64, q_stride: u64) c_int;
+pub extern "zwgpu" fn zwg_kvq_append_batch(kv: *Kvq, layer: u64, seq0: u64, n_seq: u64, pos_dev: [*]const i32,
+    rope_pos_dev: ?[*]const i32, k_rows: [*]const f32, v_rows: [*]const f32, q: ?[*]const f32, q_out: ?[*]f32,
+    n_head: u64, q_stride: u64) c_int;
+pub extern "zwgpu" fn zwg_kvq_rows_dev(kv: *Kvq, layer0: u64, n_layer: u64, seq0: u64, n_seq: u64,
+    pos_dev: ?[*]const i32, pos0: u64, n: u64, k_out: ?[*]f32, v_out: ?[*]f32) c_int;
+pub extern "zwgpu" fn zwg_kvq_attention_dev(kv: *Kvq, layer: u64, seq0: u64, n_seq: u64, q: [*]const f32,
+    attn: *const KvqAttn, out: [*]f32, weights: ?[*]f32) c_int;
+pub extern "zwgpu" fn zwg_kvq_evict_dev(kv: *Kvq, layer0: u64, n_layer: u64, seq0: u64, n_seq: u64, cut: *const KvqCut,
+    weights: ?[*]const f32, weights_out: ?[*]f32) c_int;
+
 // ---- the calling thread's context
 
 /// One context per thread that calls into ops (the zw_* handles are per thread too,

@@ -147,6 +147,65 @@ class KVInfoC(ctypes.Structure):
     ]
 
 
+class RopeDescC(ctypes.Structure):
+    _fields_ = [
+        ("n_ctx", _u64),
+        ("d", _u64),
+        ("n_rot", _u64),
+        ("layout", ctypes.c_uint32),
+        ("scaling", ctypes.c_uint32),
+        ("base", ctypes.c_double),
+        ("factor", ctypes.c_double),
+        ("n_orig", _u64),
+        ("beta_fast", ctypes.c_double),
+        ("beta_slow", ctypes.c_double),
+        ("mscale", ctypes.c_double),
+    ]
+
+
+class KVQDescC(ctypes.Structure):
+    _fields_ = [
+        ("n_layer", _u64),
+        ("n_seq", _u64),
+        ("n_ctx", _u64),
+        ("n_head_kv", _u64),
+        ("d", _u64),
+        ("block", _u64),
+        ("format", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class KVQAttnC(ctypes.Structure):
+    _fields_ = [
+        ("n_q", _u64),
+        ("n_kv", _u64),
+        ("n_head", _u64),
+        ("q_stride", _u64),
+        ("out_stride", _u64),
+        ("q_bstride", _u64),
+        ("out_bstride", _u64),
+        ("weights_stride", _u64),
+        ("weights_bstride", _u64),
+        ("n_kv_dev", ctypes.c_void_p),
+        ("decay", ctypes.c_float),
+        ("causal", ctypes.c_uint32),
+    ]
+
+
+class KVQCutC(ctypes.Structure):
+    _fields_ = [
+        ("n_kv", _u64),
+        ("n_keep", _u64),
+        ("n_first", _u64),
+        ("n_recent", _u64),
+        ("weights_stride", _u64),
+        ("n_kv_dev", ctypes.c_void_p),
+        ("n_kv_out", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+    ]
+
+
 DENSE_X3 = 0
 DENSE_FP32 = 1
 KV_ROW = 0
@@ -158,6 +217,15 @@ EPI_NONE = 0
 EPI_GELU = 1
 EPI_ADD = 2
 ROWS_ON_HOST = 1
+ROPE_HALF = 0
+ROPE_INTERLEAVED = 1
+ROPE_NONE = 0
+ROPE_LINEAR = 1
+ROPE_NTK = 2
+ROPE_YARN = 3
+ROPE_INVERSE = 1
+KVQ_I8 = 0
+KVQ_E4M3 = 1
 NOALLOC_SCRATCH_BYTES = 64 << 20  # ZWG_NOALLOC_SCRATCH_BYTES
 
 
@@ -221,6 +289,28 @@ def lib() -> ctypes.CDLL:
     L.zwg_kv_append_batch.argtypes = [vp, _u64, _u64, _u64, vp, _fp, _fp, _fp, _u64, _u64]
     L.zwg_kv_read.restype = c_int
     L.zwg_kv_read.argtypes = [vp, _u64, _u64, _fp, _fp]
+    L.zwg_rope_create.restype = c_int
+    L.zwg_rope_create.argtypes = [vp, ctypes.POINTER(RopeDescC), ctypes.POINTER(vp)]
+    L.zwg_rope_destroy.restype = None
+    L.zwg_rope_destroy.argtypes = [vp]
+    L.zwg_rope_apply_dev.restype = c_int
+    L.zwg_rope_apply_dev.argtypes = [vp, _fp, _u64, _u64, _u64, vp, _u64, _fp, _u64, ctypes.c_uint32]
+    L.zwg_kvq_create.restype = c_int
+    L.zwg_kvq_create.argtypes = [vp, ctypes.POINTER(KVQDescC), vp, ctypes.POINTER(vp)]
+    L.zwg_kvq_destroy.restype = None
+    L.zwg_kvq_destroy.argtypes = [vp]
+    L.zwg_kvq_bytes.restype = _u64
+    L.zwg_kvq_bytes.argtypes = [ctypes.POINTER(KVQDescC)]
+    L.zwg_kvq_append.restype = c_int
+    L.zwg_kvq_append.argtypes = [vp, _u64, _u64, _u64, _u64, _u64, _fp, _fp, _fp, _fp, _u64, _u64]
+    L.zwg_kvq_append_batch.restype = c_int
+    L.zwg_kvq_append_batch.argtypes = [vp, _u64, _u64, _u64, vp, vp, _fp, _fp, _fp, _fp, _u64, _u64]
+    L.zwg_kvq_rows_dev.restype = c_int
+    L.zwg_kvq_rows_dev.argtypes = [vp, _u64, _u64, _u64, _u64, vp, _u64, _u64, _fp, _fp]
+    L.zwg_kvq_attention_dev.restype = c_int
+    L.zwg_kvq_attention_dev.argtypes = [vp, _u64, _u64, _u64, _fp, ctypes.POINTER(KVQAttnC), _fp, _fp]
+    L.zwg_kvq_evict_dev.restype = c_int
+    L.zwg_kvq_evict_dev.argtypes = [vp, _u64, _u64, _u64, _u64, ctypes.POINTER(KVQCutC), _fp, _fp]
     for name in ("zwg_linear", "zwg_linear_dev"):
         getattr(L, name).restype = c_int
         getattr(L, name).argtypes = [vp, _fp, _u64, _u64, vp, ctypes.c_uint32, _fp, _u64, _fp]

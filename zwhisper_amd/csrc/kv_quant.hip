@@ -1,0 +1,755 @@
+// Writing and reading the 8-bit key/value caches (include/zw_gpu.h, zwg_kvq_*): appends, reads as values, eviction.
+//
+// A block's scale is shared by all its tokens, so a token that outgrows it changes the codes of every token
+// before it in the block.  The rows of the block being filled are therefore also held in f32: the codes are always
+// those of the block's rows, never codes of codes.  An appended token whose block keeps its largest
+// magnitude (most do: token r of a block brings a new largest one time in r + 1) writes its own codes alone.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "kv_quant.hpp"
+#include "zw_ctx.hpp"
+
+using namespace zwg_host;
+using namespace zwg_planner;
+using zwg::KvqOpen;
+using zwg::KvqView;
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kPad = 4; // floats between the staged rows' ends and the next row: 16-byte rows on other banks
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+struct AppendArgs {
+    KvqView view;
+    zwg::RopeView rope;
+    int64_t unit0; // unit of (layer, seq0, head 0)
+    const float *src[2]; // [n][n_head_kv * d]
+    const float *q;
+    float *q_out;
+    int64_t q_stride;
+    const int32_t *pos_dev, *rope_pos_dev; // one token per sequence; nullptr: n tokens of one, at pos0 and rope_pos0
+    int64_t pos0, rope_pos0;
+    int32_t n, n_head;
+};
+
+// Codes of rows [r0, r1) of the staged block in `rows`, written to the unit's codes.  16 rows of a value
+// tile's dim are four runs of four bytes, so both tensors are written in words of four codes; the rows of a
+// word outside [r0, r1) are written only where the whole block is (r0 = 0, r1 = block).
+template <int D, int FMT, int IS_V>
+__device__ __forceinline__ void write_codes(uint8_t *codes, const float (*rows)[D + kPad], int block_size, int64_t first,
+                                            int r0, int r1, float mul) {
+    if (!IS_V) {
+        for (int i = threadIdx.x; i < (r1 - r0) * (D / 4); i += kAppendThreads) {
+            const int r = r0 + i / (D / 4), c = 4 * (i % (D / 4));
+            const float4 x = *reinterpret_cast<const float4 *>(&rows[r][c]);
+            *reinterpret_cast<uint32_t *>(codes + (first + r) * D + c) = zwg::kvq_encode4<FMT>(x.x, x.y, x.z, x.w, mul);
+        }
+    } else if (r0 == 0 && r1 == block_size) {
+        for (int i = threadIdx.x; i < block_size / 4 * D; i += kAppendThreads) {
+            const int c = i % D, r = 4 * (i / D);
+            *reinterpret_cast<uint32_t *>(codes + zwg::kvq_at(1, first + r, c, D)) =
+                zwg::kvq_encode4<FMT>(rows[r][c], rows[r + 1][c], rows[r + 2][c], rows[r + 3][c], mul);
+        }
+    } else {
+        for (int i = threadIdx.x; i < (r1 - r0) * D; i += kAppendThreads) {
+            const int r = r0 + i / D, c = i % D;
+            codes[zwg::kvq_at(1, first + r, c, D)] = (uint8_t)zwg::kvq_encode4<FMT>(rows[r][c], 0.f, 0.f, 0.f, mul);
+        }
+    }
+}
+
+// One block of a unit: rows [r0, r1) are new (token `tok` on), those before r0 are held in the open block or
+// count as the values of their codes, those from r1 on become zeros.  keep: the block stays open (it is the last
+// that the call touches).
+template <int D, int FMT, int IS_V>
+__device__ void append_block(const AppendArgs &a, int64_t u, int head, int b, int r0, int r1, int64_t tok,
+                             int64_t rope_pos, bool keep, float (*rows)[D + kPad], uint32_t *top, uint32_t *shared_top) {
+    const KvqView &v = a.view;
+    const int B = v.block, tid = threadIdx.x;
+    const int kvw = v.n_head_kv * D;
+    uint8_t *codes = v.codes[IS_V] + u * v.unit_bytes;
+    float *scale_at = v.scales[IS_V] + u * v.n_blocks + b;
+    float *held = v.rows[IS_V] + u * B * D;
+    KvqOpen *open = v.open + 2 * u + IS_V;
+    const int64_t first = (int64_t)b * B;
+
+    const bool is_open = open->block == b;
+    const int filled = is_open ? open->filled : 0;
+    const float old_scale = *scale_at;
+    // the new rows, rotated
+    for (int i = tid; i < (r1 - r0) * (D / 4); i += kAppendThreads) {
+        const int r = i / (D / 4), c = 4 * (i % (D / 4));
+        *reinterpret_cast<float4 *>(&rows[r0 + r][c]) =
+            *reinterpret_cast<const float4 *>(a.src[IS_V] + (tok + r) * kvw + head * D + c);
+    }
+    if (tid < B) top[tid] = tid < r0 && tid < filled ? abs_bits(open->top[tid]) : 0u;
+    __syncthreads();
+    if (!IS_V && a.rope.cos) {
+        const int turned = zwg::rope_turned(a.rope);
+        for (int i = tid; i < (r1 - r0) * turned; i += kAppendThreads) {
+            const int r = i / turned;
+            zwg::rope_piece(a.rope, rope_pos + r, i - r * turned, rows[r0 + r], rows[r0 + r]);
+        }
+        __syncthreads();
+    }
+    // each row's largest magnitude: D / 4 lanes a row (8, 16 or 32, in one wave)
+    for (int i = tid; i < (r1 - r0) * (D / 4); i += kAppendThreads) {
+        const int r = r0 + i / (D / 4), c = 4 * (i % (D / 4));
+        const float4 x = *reinterpret_cast<const float4 *>(&rows[r][c]);
+        uint32_t m = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
+#pragma unroll
+        for (int off = D / 8; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
+        if (i % (D / 4) == 0) top[r] = m;
+    }
+    __syncthreads();
+    if (tid < 64) {
+        uint32_t m = tid < r1 ? top[tid] : 0u, was = tid < filled ? abs_bits(open->top[tid]) : 0u;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            m = max(m, (uint32_t)__shfl_xor((int)m, off));
+            was = max(was, (uint32_t)__shfl_xor((int)was, off));
+        }
+        if (tid == 0) {
+            shared_top[0] = m;
+            shared_top[1] = was;
+        }
+    }
+    __syncthreads();
+    float scale, mul;
+    zwg::kvq_scale<FMT>(shared_top[0], &scale, &mul);
+    // an open block whose largest magnitude stays, with no row behind r1 to clear, needs the new rows' codes
+    // alone (rows between the filled ones and r0 are zeros already)
+    const bool same = is_open && filled <= r1 && shared_top[0] == shared_top[1];
+    if (same) {
+        write_codes<D, FMT, IS_V>(codes, rows, B, first, r0, r1, mul);
+    } else {
+        // the whole block: the rows before r0, then zeros behind r1
+        for (int i = tid; i < r0 * (D / 4); i += kAppendThreads) {
+            const int r = i / (D / 4), c = 4 * (i % (D / 4));
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (is_open) {
+                if (r < filled) x = *reinterpret_cast<const float4 *>(held + r * D + c);
+            } else {
+                x.x = zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(IS_V, first + r, c, D)]) * old_scale;
+                x.y = zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(IS_V, first + r, c + 1, D)]) * old_scale;
+                x.z = zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(IS_V, first + r, c + 2, D)]) * old_scale;
+                x.w = zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(IS_V, first + r, c + 3, D)]) * old_scale;
+            }
+            *reinterpret_cast<float4 *>(&rows[r][c]) = x;
+        }
+        for (int i = tid; i < (B - r1) * (D / 4); i += kAppendThreads) {
+            const int r = r1 + i / (D / 4), c = 4 * (i % (D / 4));
+            *reinterpret_cast<float4 *>(&rows[r][c]) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        __syncthreads(); // also: every old code is read before any is written
+        if (!is_open && r0 > 0) {
+            // the reopened rows take part in the block's largest magnitude
+            for (int i = tid; i < r0 * (D / 4); i += kAppendThreads) {
+                const int r = i / (D / 4), c = 4 * (i % (D / 4));
+                const float4 x = *reinterpret_cast<const float4 *>(&rows[r][c]);
+                uint32_t m = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
+#pragma unroll
+                for (int off = D / 8; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
+                if (i % (D / 4) == 0) top[r] = m;
+            }
+            __syncthreads();
+            if (tid < 64) {
+                uint32_t m = tid < r1 ? top[tid] : 0u;
+#pragma unroll
+                for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
+                if (tid == 0) shared_top[0] = m;
+            }
+            __syncthreads();
+            zwg::kvq_scale<FMT>(shared_top[0], &scale, &mul);
+        }
+        write_codes<D, FMT, IS_V>(codes, rows, B, first, 0, B, mul);
+        if (tid == 0) *scale_at = scale;
+    }
+    if (keep) {
+        // rows of an open block that was held already stay where they are; gap rows (filled .. r0) are zeros
+        const int from = is_open ? min(filled, r0) : 0;
+        if (same && from < r0) {
+            for (int i = tid; i < (r0 - from) * (D / 4); i += kAppendThreads)
+                *reinterpret_cast<float4 *>(&rows[from + i / (D / 4)][4 * (i % (D / 4))]) = make_float4(0.f, 0.f, 0.f, 0.f);
+            __syncthreads();
+        }
+        for (int i = tid; i < (r1 - from) * (D / 4); i += kAppendThreads) {
+            const int r = from + i / (D / 4), c = 4 * (i % (D / 4));
+            *reinterpret_cast<float4 *>(held + r * D + c) = *reinterpret_cast<const float4 *>(&rows[r][c]);
+        }
+        if (tid < r1) open->top[tid] = __builtin_bit_cast(float, top[tid]);
+        if (tid == 0) {
+            open->block = b;
+            open->filled = r1;
+        }
+    }
+    __syncthreads(); // the staging may be used for another block
+}
+
+// Workgroups (x, y): y < 2 n_head_kv: head y / 2's keys (y even) or values of the x-th touched block (tokens of one
+// sequence) or of sequence x (one token each); from there on query head y - 2 n_head_kv of the same tokens.
+// The first and the last block of one call both deal with the unit's open block, so one workgroup does them in
+// turn, and a call that touches m blocks has m - 1 of them (at least one).
+template <int D, int FMT> __global__ __launch_bounds__(kAppendThreads) void kvq_append_kernel(AppendArgs a) {
+    __shared__ __align__(16) float rows[zwg::kKvqMaxBlock][D + kPad];
+    __shared__ uint32_t top[zwg::kKvqMaxBlock];
+    __shared__ uint32_t shared_top[2];
+    const KvqView &v = a.view;
+    const int B = v.block, x = blockIdx.x, y = blockIdx.y;
+
+    int64_t pos = a.pos0, rp = a.rope_pos0, n = a.n, tok = 0, u = a.unit0;
+    if (a.pos_dev) {
+        pos = a.pos_dev[x];
+        rp = a.rope_pos_dev ? a.rope_pos_dev[x] : pos;
+        if (pos < 0 || pos >= v.n_ctx || (a.rope.cos && (rp < 0 || rp >= a.rope.n_ctx))) return;
+        n = 1;
+        tok = x;
+        u += (int64_t)x * v.n_head_kv;
+    }
+    const int64_t b0 = pos / B, b1 = (pos + n - 1) / B;
+
+    if (y >= 2 * v.n_head_kv) {
+        // query rows: B tokens a workgroup, as if from the start of the first block
+        const int h = y - 2 * v.n_head_kv;
+        const int pieces = a.q == a.q_out ? zwg::rope_turned(a.rope) : zwg::rope_pieces(a.rope);
+        // with one workgroup less than blocks, the first takes the last block's tokens too
+        for (int64_t b = b0 + (a.pos_dev ? 0 : x); b <= b1; b += b1 - b0) {
+            const int64_t t0 = max(pos, b * B) - pos, t1 = min(pos + n, (b + 1) * B) - pos;
+            for (int i = threadIdx.x; i < (int)(t1 - t0) * pieces; i += kAppendThreads) {
+                const int t = i / pieces, c = i - t * pieces;
+                const int64_t row = (tok + t0 + t) * a.q_stride + (int64_t)h * D;
+                zwg::rope_piece(a.rope, rp + t0 + t, c, a.q + row, a.q_out + row);
+            }
+            if (b != b0 || b1 == b0) break;
+        }
+        return;
+    }
+    const int head = y >> 1;
+    u += head;
+    for (int64_t b = b0 + (a.pos_dev ? 0 : x); b <= b1; b += b1 - b0) {
+        const int64_t t0 = max(pos, b * B) - pos, t1 = min(pos + n, (b + 1) * B) - pos;
+        const int r0 = (int)(pos + t0 - b * B), r1 = (int)(pos + t1 - b * B);
+        if (y & 1)
+            append_block<D, FMT, 1>(a, u, head, (int)b, r0, r1, tok + t0, rp + t0, b == b1, rows, top, shared_top);
+        else
+            append_block<D, FMT, 0>(a, u, head, (int)b, r0, r1, tok + t0, rp + t0, b == b1, rows, top, shared_top);
+        if (b != b0 || b1 == b0) break;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- reads
+
+struct RowsArgs {
+    KvqView view;
+    int64_t layer0, seq0;
+    const int32_t *pos_dev;
+    int64_t pos0;
+    int64_t n; // positions of a sequence
+    int32_t n_seq;
+    float *out[2]; // [n_layer][n_seq][n][n_head_kv * d]
+};
+
+// Workgroups (x, y, z): 32 positions from 32 x of (layer, sequence) y; z: KV head and keys or values.
+template <int D, int FMT> __global__ __launch_bounds__(256) void kvq_rows_kernel(RowsArgs a) {
+    const KvqView &v = a.view;
+    const int is_v = blockIdx.z & 1, head = blockIdx.z >> 1;
+    float *out = a.out[is_v];
+    if (!out) return;
+    const int64_t layer = a.layer0 + blockIdx.y / a.n_seq, i = blockIdx.y % a.n_seq;
+    const int64_t u = (layer * v.n_seq + a.seq0 + i) * v.n_head_kv + head;
+    const uint8_t *codes = v.codes[is_v] + u * v.unit_bytes;
+    const float *scales = v.scales[is_v] + u * v.n_blocks;
+    const int64_t start = a.pos_dev ? (int64_t)a.pos_dev[i] : a.pos0;
+    const int kvw = v.n_head_kv * D;
+    for (int k = threadIdx.x; k < 32 * D; k += 256) {
+        const int64_t t = (int64_t)blockIdx.x * 32 + k / D;
+        const int c = k % D;
+        const int64_t p = start + t;
+        if (t >= a.n || p < 0 || p >= v.n_ctx) continue;
+        out[((int64_t)blockIdx.y * a.n + t) * kvw + head * D + c] =
+            zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(is_v, p, c, D)]) * scales[p / v.block];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- eviction
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWaves = kSelectThreads / 64;
+
+struct CutArgs {
+    KvqView view;
+    int64_t layer0, seq0;
+    int32_t n_seq, n_layer;
+    int32_t n_kv, n_keep, n_first, n_recent;
+    int64_t w_stride;
+    const int32_t *n_kv_dev;
+    int32_t *n_kv_out, *kept;
+    const float *w;
+    float *w_out;
+    int32_t *src;   // [unit of the call][n_keep]: the kept tokens' old positions
+    int32_t *count; // [unit of the call]: the tokens before the cut (the counts may be overwritten after it)
+};
+
+// A weight as an unsigned number in the order of the selection: negative below positive, the zeros equal, a NaN
+// above everything.
+__device__ __forceinline__ uint32_t rank_bits(float w) {
+    if (w != w) return 0xffffffffu;
+    const uint32_t b = __builtin_bit_cast(uint32_t, w + 0.0f); // -0 + 0 = 0
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// One workgroup per (layer, sequence, head): the threshold weight by four passes over 8 bits each (counts in
+// LDS, whole numbers, so their order does not matter), then one ordered pass that writes the kept positions
+// and weights.  Equal weights at the threshold go to the lowest positions.
+__global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t found_prefix, found_left;
+    __shared__ int wave_more[kSelectWaves], wave_ties[kSelectWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t cu = blockIdx.x; // unit of the call
+    const int H = a.view.n_head_kv;
+    const int seq = (int)((cu / H) % a.n_seq);
+    const int n = a.n_kv_dev ? min(max(a.n_kv_dev[seq], 0), a.n_kv) : a.n_kv;
+    const float *w = a.w + cu * a.w_stride;
+    float *w_out = a.w_out ? a.w_out + cu * a.w_stride : nullptr;
+    int32_t *src = a.src + cu * a.n_keep;
+    int32_t *kept = a.kept ? a.kept + cu * a.n_keep : nullptr;
+    if (tid == 0) a.count[cu] = n;
+    if (n <= a.n_keep) {
+        for (int i = tid; i < a.n_keep; i += kSelectThreads)
+            if (kept) kept[i] = i < n ? i : -1;
+        if (w_out)
+            for (int i = tid; i < a.n_kv; i += kSelectThreads) w_out[i] = i < n ? w[i] : 0.0f;
+        return;
+    }
+    const int lo = a.n_first, hi = n - a.n_recent; // the contested positions
+    uint32_t prefix = 0, left = (uint32_t)(a.n_keep - a.n_first - a.n_recent); // < hi - lo
+#pragma unroll 1
+    for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int i = lo + tid; i < hi; i += kSelectThreads) {
+            const uint32_t r = rank_bits(w[i]);
+            if (shift == 24 || (r >> (shift + 8)) == prefix) atomicAdd(&hist[(r >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // the digit at which the counts from the top reach `left`: four digits a lane, lane 0 the highest
+            uint32_t c[4], s = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                c[k] = hist[255 - 4 * lane - k];
+                s += c[k];
+            }
+            uint32_t incl = s;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t o = (uint32_t)__shfl_up((int)incl, off);
+                if (lane >= off) incl += o;
+            }
+            uint32_t before = incl - s;
+            if (before < left && incl >= left) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (before < left && before + c[k] >= left) {
+                        found_prefix = (prefix << 8) | (uint32_t)(255 - 4 * lane - k);
+                        found_left = left - before;
+                    }
+                    before += c[k];
+                }
+            }
+        }
+        __syncthreads();
+        prefix = found_prefix;
+        left = found_left;
+        __syncthreads();
+    }
+    // now `prefix` is the threshold and `left` of its equals stay (none contested: nothing stays between)
+    const bool any = a.n_keep > a.n_first + a.n_recent;
+    int done = 0, ties = 0; // kept so far, and ties met so far
+    for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
+        const int i = i0 + tid;
+        float wi = 0.0f;
+        bool more = false, tie = false;
+        if (i < n) {
+            wi = w[i];
+            const uint32_t r = rank_bits(wi);
+            const bool fixed = i < lo || i >= hi;
+            more = fixed || (any && r > prefix);
+            tie = !fixed && any && r == prefix;
+        }
+        const unsigned long long tb = __ballot(tie);
+        if (lane == 0) wave_ties[wave] = __popcll(tb);
+        __syncthreads();
+        int t = ties;
+        for (int k = 0; k < kSelectWaves; ++k) {
+            const int c = wave_ties[k];
+            if (k < wave) t += c;
+            ties += c;
+        }
+        t += __popcll(tb & ((1ull << lane) - 1));
+        const bool stays = more || (tie && (uint32_t)t < left);
+        const unsigned long long sb = __ballot(stays);
+        if (lane == 0) wave_more[wave] = __popcll(sb);
+        __syncthreads();
+        int at = done;
+        for (int k = 0; k < kSelectWaves; ++k) {
+            const int c = wave_more[k];
+            if (k < wave) at += c;
+            done += c;
+        }
+        at += __popcll(sb & ((1ull << lane) - 1));
+        // every weight of these positions is read (it decided `stays`, which the barrier above follows), and new
+        // positions never lie above old ones: the weights may be compacted in place
+        if (stays) {
+            src[at] = i;
+            if (kept) kept[at] = i;
+            if (w_out) w_out[at] = wi;
+        }
+        __syncthreads();
+    }
+    if (w_out)
+        for (int i = a.n_keep + tid; i < a.n_kv; i += kSelectThreads) w_out[i] = 0.0f;
+}
+
+constexpr int kMoveThreads = 1024;
+
+// One workgroup per (layer, sequence, head) and keys or values: new blocks in groups, in ascending order.  A
+// kept token never moves up, so the tokens of a group and all later ones lie at or above the group's first position:
+// once a group's codes are in registers (their magnitudes, which depend on them, are in LDS before the
+// barrier) its positions may be overwritten, and no later group misses what was there.
+template <int D, int FMT> __global__ __launch_bounds__(kMoveThreads) void kvq_move_kernel(CutArgs a) {
+    constexpr int kWords = 16;                         // words of four codes in a thread's registers
+    constexpr int kGroup = kMoveThreads * kWords * 4 / D; // tokens of a group: 2048 at d = 32 down to 512
+    __shared__ uint32_t tops[kGroup / 16];
+    const KvqView &v = a.view;
+    const int tid = threadIdx.x;
+    const int64_t cu = blockIdx.x >> 1;
+    const int is_v = blockIdx.x & 1;
+    const int H = v.n_head_kv, B = v.block;
+    const int64_t layer = a.layer0 + cu / ((int64_t)H * a.n_seq);
+    const int64_t seq = (cu / H) % a.n_seq, head = cu % H;
+    const int n = a.count[cu];
+    if (is_v && cu % H == 0 && cu / H < a.n_seq && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
+    if (n <= a.n_keep) return;
+    const int64_t u = (layer * v.n_seq + a.seq0 + seq) * H + head;
+    uint8_t *codes = v.codes[is_v] + u * v.unit_bytes;
+    float *scales = v.scales[is_v] + u * v.n_blocks;
+    const int32_t *src = a.src + cu * a.n_keep;
+    if (tid == 0) v.open[2 * u + is_v].block = -1; // the open block's rows are others now
+    const int end = (a.n_keep + B - 1) / B * B;
+#pragma unroll 1
+    for (int t0 = 0; t0 < end; t0 += kGroup) {
+        if (tid < kGroup / 16) tops[tid] = 0;
+        __syncthreads();
+        // word k of a thread: keys: token t0 + w / (D / 4), dims 4 (w % (D / 4)) ..; values: dim w % D of tokens
+        // t0 + 4 (w / D) ..; w = k * threads + tid
+        float x[kWords][4];
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            const int w = k * kMoveThreads + tid;
+            uint32_t top = 0;
+            int first;
+            if (!is_v) {
+                const int t = t0 + w / (D / 4), c = 4 * (w % (D / 4));
+                first = t;
+                uint32_t word = 0;
+                float s = 0.0f;
+                if (t < a.n_keep) {
+                    const int p = src[t];
+                    word = *reinterpret_cast<const uint32_t *>(codes + (int64_t)p * D + c);
+                    s = scales[p / B];
+                }
+                x[k][0] = t < a.n_keep ? zwg::kvq_decode<FMT, 0>(word) * s : 0.0f;
+                x[k][1] = t < a.n_keep ? zwg::kvq_decode<FMT, 1>(word) * s : 0.0f;
+                x[k][2] = t < a.n_keep ? zwg::kvq_decode<FMT, 2>(word) * s : 0.0f;
+                x[k][3] = t < a.n_keep ? zwg::kvq_decode<FMT, 3>(word) * s : 0.0f;
+            } else {
+                const int t = t0 + 4 * (w / D), c = w % D;
+                first = t;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[k][e] = 0.0f;
+                    if (t + e < a.n_keep) {
+                        const int p = src[t + e];
+                        x[k][e] = zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(1, p, c, D)]) * scales[p / B];
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, abs_bits(x[k][e]));
+            // a wave's 64 words are of at most 8 aligned tokens: of one block
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+            if ((tid & 63) == 0 && first < end) atomicMax(&tops[(first - t0) / B], top);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            const int w = k * kMoveThreads + tid;
+            const int t = is_v ? t0 + 4 * (w / D) : t0 + w / (D / 4);
+            if (t >= end) continue;
+            float scale, mul;
+            zwg::kvq_scale<FMT>(tops[(t - t0) / B], &scale, &mul);
+            const uint32_t word = zwg::kvq_encode4<FMT>(x[k][0], x[k][1], x[k][2], x[k][3], mul);
+            const int c = is_v ? w % D : 4 * (w % (D / 4));
+            *reinterpret_cast<uint32_t *>(codes + zwg::kvq_at(is_v, t, c, D)) = word;
+            if (c == 0 && t % B == 0) scales[t / B] = scale;
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+
+const char *const kKvqClosed = "the kvq cache's context is closed";
+
+void release(zwg_kvq *kv) {
+    if (kv->ctx) {
+        (void)hipSetDevice(kv->ctx->device);
+        (void)hipStreamSynchronize(kv->ctx->stream);
+    }
+    if (kv->mem) (void)hipFree(kv->mem);
+    kv->mem = nullptr;
+    kv->tables.reset();
+}
+
+void detach_kvq(void *obj) {
+    auto *kv = static_cast<zwg_kvq *>(obj);
+    release(kv);
+    kv->ctx = nullptr;
+}
+
+int create(zwg_ctx *ctx, const zwg_kvq_desc *desc, const zwg_rope *rope, zwg_kvq **out) {
+    const std::string msg = check_kvq_desc(*desc);
+    if (!msg.empty()) return fail(ctx, msg);
+    if (rope) {
+        if (rope->ctx != ctx) return fail(ctx, "the rope belongs to another context (or its context is closed)");
+        if (rope->desc.d != desc->d) return fail(ctx, "the rope's head dim differs from the cache's");
+    }
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return fail_hip(ctx, "hipSetDevice", e);
+    const KvqLayout l = kvq_layout(*desc);
+    auto kv = std::make_unique<zwg_kvq>();
+    kv->ctx = ctx;
+    kv->desc = *desc;
+    kv->n_pad = l.n_pad;
+    e = hipMalloc(&kv->mem, l.total);
+    if (e != hipSuccess) {
+        kv->mem = nullptr;
+        return fail_hip(ctx, "kvq cache allocation", e);
+    }
+    uint8_t *p = static_cast<uint8_t *>(kv->mem);
+    KvqView &v = kv->view;
+    for (int i = 0; i < 2; ++i) {
+        v.codes[i] = p;
+        p += l.codes;
+    }
+    for (int i = 0; i < 2; ++i) {
+        v.scales[i] = reinterpret_cast<float *>(p);
+        p += l.scales;
+    }
+    for (int i = 0; i < 2; ++i) {
+        v.rows[i] = reinterpret_cast<float *>(p);
+        p += l.rows;
+    }
+    v.open = reinterpret_cast<KvqOpen *>(p);
+    v.unit_bytes = (int64_t)(l.n_pad * desc->d);
+    v.n_blocks = (int32_t)(l.n_pad / desc->block);
+    v.block = (int32_t)desc->block;
+    v.n_ctx = (int32_t)desc->n_ctx;
+    v.d = (int32_t)desc->d;
+    v.n_head_kv = (int32_t)desc->n_head_kv;
+    v.n_seq = (int32_t)desc->n_seq;
+    // zeros: the code of zero, zero scales, no open block (-1)
+    e = hipMemsetAsync(v.codes[0], desc->format == ZWG_KVQ_I8 ? 0x80 : 0, 2 * l.codes, ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(v.scales[0], 0, 2 * (l.scales + l.rows), ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(v.open, 0xff, l.open, ctx->stream);
+    const hipError_t es = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess) e = es;
+    if (e != hipSuccess) {
+        release(kv.get());
+        return fail_hip(ctx, "kvq cache", e);
+    }
+    if (rope) {
+        kv->has_rope = true;
+        kv->rope = rope->desc;
+        kv->tables = rope->tables;
+    }
+    add_child(ctx, kv.get(), detach_kvq);
+    *out = kv.release();
+    return ZWG_OK;
+}
+
+#define ZWG_KVQ_DISPATCH(KERNEL, D_, FMT_, ...)                                                                   \
+    switch (D_) {                                                                                                \
+    case 32: if (FMT_ == ZWG_KVQ_I8) KERNEL<32, 0> __VA_ARGS__; else KERNEL<32, 1> __VA_ARGS__; break;            \
+    case 64: if (FMT_ == ZWG_KVQ_I8) KERNEL<64, 0> __VA_ARGS__; else KERNEL<64, 1> __VA_ARGS__; break;            \
+    default: if (FMT_ == ZWG_KVQ_I8) KERNEL<128, 0> __VA_ARGS__; else KERNEL<128, 1> __VA_ARGS__; break;          \
+    }
+
+int append(zwg_kvq *kv, const KvqAppend &c, float *q_out) {
+    zwg_ctx *ctx = kv->ctx;
+    const zwg_kvq_desc &d = kv->desc;
+    const std::string msg = check_kvq_append(d, kv->has_rope ? &kv->rope : nullptr, c);
+    if (!msg.empty()) return fail(ctx, msg);
+    if (c.n == 0) return ZWG_OK;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return fail_hip(ctx, "hipSetDevice", e);
+    AppendArgs a{};
+    a.view = kv->view;
+    if (kv->has_rope) a.rope = zwg::rope_view(kv->rope, *kv->tables, false);
+    a.unit0 = (int64_t)((c.layer * d.n_seq + c.seq0) * d.n_head_kv);
+    a.src[0] = c.k;
+    a.src[1] = c.v;
+    a.q = c.q;
+    a.q_out = q_out;
+    a.q_stride = (int64_t)c.q_stride;
+    a.pos_dev = c.batch ? c.pos_dev : nullptr;
+    a.rope_pos_dev = c.batch ? c.rope_pos_dev : nullptr;
+    a.pos0 = (int64_t)c.pos;
+    a.rope_pos0 = (int64_t)c.rope_pos;
+    a.n = (int32_t)c.n;
+    a.n_head = (int32_t)c.n_head;
+    const uint64_t blocks = c.batch ? c.n : std::max<uint64_t>(1, (c.pos + c.n - 1) / d.block - c.pos / d.block);
+    const dim3 grid((unsigned)blocks, (unsigned)(2 * d.n_head_kv + (c.q ? c.n_head : 0)));
+    ZWG_KVQ_DISPATCH(kvq_append_kernel, d.d, d.format, <<<grid, kAppendThreads, 0, ctx->stream>>>(a))
+    e = hipGetLastError();
+    return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "kvq append launch", e);
+}
+
+int rows(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq, const int32_t *pos_dev,
+         uint64_t pos0, uint64_t n, float *k_out, float *v_out) {
+    zwg_ctx *ctx = kv->ctx;
+    const zwg_kvq_desc &d = kv->desc;
+    const std::string msg = check_kvq_rows(d, layer0, n_layer, seq0, n_seq, pos_dev, pos0, n, k_out, v_out);
+    if (!msg.empty()) return fail(ctx, msg);
+    if (n_layer == 0 || n_seq == 0 || n == 0 || (!k_out && !v_out)) return ZWG_OK;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return fail_hip(ctx, "hipSetDevice", e);
+    RowsArgs a{};
+    a.view = kv->view;
+    a.layer0 = (int64_t)layer0;
+    a.seq0 = (int64_t)seq0;
+    a.pos_dev = pos_dev;
+    a.pos0 = (int64_t)pos0;
+    a.n = (int64_t)n;
+    a.n_seq = (int32_t)n_seq;
+    a.out[0] = k_out;
+    a.out[1] = v_out;
+    const dim3 grid((unsigned)((n + 31) / 32), (unsigned)(n_layer * n_seq), (unsigned)(2 * d.n_head_kv));
+    ZWG_KVQ_DISPATCH(kvq_rows_kernel, d.d, d.format, <<<grid, 256, 0, ctx->stream>>>(a))
+    e = hipGetLastError();
+    return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "kvq rows launch", e);
+}
+
+int evict(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq, const zwg_kvq_cut *c,
+          const float *weights, float *weights_out) {
+    zwg_ctx *ctx = kv->ctx;
+    const zwg_kvq_desc &d = kv->desc;
+    const std::string msg = check_kvq_cut(d, layer0, n_layer, seq0, n_seq, *c, weights, weights_out);
+    if (!msg.empty()) return fail(ctx, msg);
+    if (n_layer == 0 || n_seq == 0) return ZWG_OK;
+    const uint64_t units = n_layer * n_seq * d.n_head_kv, need = kvq_cut_bytes(units, *c);
+    if (need > ctx->workspace_bytes) {
+        char buf[200];
+        snprintf(buf, sizeof buf, "this eviction lists %llu bytes of kept positions, more than the context's workspace (%llu): fewer layers or sequences a call",
+                 (unsigned long long)need, (unsigned long long)ctx->workspace_bytes);
+        return fail(ctx, buf);
+    }
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return fail_hip(ctx, "hipSetDevice", e);
+    CutArgs a{};
+    a.view = kv->view;
+    a.layer0 = (int64_t)layer0;
+    a.seq0 = (int64_t)seq0;
+    a.n_seq = (int32_t)n_seq;
+    a.n_layer = (int32_t)n_layer;
+    a.n_kv = (int32_t)c->n_kv;
+    a.n_keep = (int32_t)c->n_keep;
+    a.n_first = (int32_t)c->n_first;
+    a.n_recent = (int32_t)c->n_recent;
+    a.w_stride = (int64_t)c->weights_stride;
+    a.n_kv_dev = c->n_kv_dev;
+    a.n_kv_out = c->n_kv_out;
+    a.kept = c->kept;
+    a.w = weights;
+    a.w_out = weights_out;
+    a.count = reinterpret_cast<int32_t *>(ctx->workspace);
+    a.src = a.count + units;
+    kvq_select_kernel<<<(unsigned)units, kSelectThreads, 0, ctx->stream>>>(a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return fail_hip(ctx, "kvq select launch", e);
+    ZWG_KVQ_DISPATCH(kvq_move_kernel, d.d, d.format, <<<(unsigned)(2 * units), kMoveThreads, 0, ctx->stream>>>(a))
+    e = hipGetLastError();
+    return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "kvq move launch", e);
+}
+
+} // namespace
+
+extern "C" {
+
+int zwg_kvq_create(zwg_ctx *ctx, const zwg_kvq_desc *desc, const zwg_rope *rope, zwg_kvq **out) {
+    if (!out) return fail(ctx, "null output pointer");
+    *out = nullptr;
+    if (!ctx || !desc) return fail(ctx, "null context or kvq desc");
+    return guarded(ctx, [&] { return create(ctx, desc, rope, out); });
+}
+
+void zwg_kvq_destroy(zwg_kvq *kv) {
+    if (!kv) return;
+    if (kv->ctx) remove_child(kv->ctx, kv);
+    release(kv);
+    delete kv;
+}
+
+uint64_t zwg_kvq_bytes(const zwg_kvq_desc *desc) {
+    if (!desc) return 0;
+    try {
+        return check_kvq_desc(*desc).empty() ? kvq_layout(*desc).total : 0;
+    } catch (...) {
+        return 0;
+    }
+}
+
+int zwg_kvq_append(zwg_kvq *kv, uint64_t layer, uint64_t seq, uint64_t pos, uint64_t n, uint64_t rope_pos,
+                   const float *k_rows, const float *v_rows, const float *q, float *q_out, uint64_t n_head,
+                   uint64_t q_stride) {
+    if (!kv) return fail(nullptr, "null kvq");
+    if (!kv->ctx) return fail(nullptr, kKvqClosed);
+    return guarded(kv->ctx, [&] {
+        return append(kv, {layer, seq, pos, n, rope_pos, false, nullptr, nullptr, k_rows, v_rows, q, q_out, n_head, q_stride}, q_out);
+    });
+}
+
+int zwg_kvq_append_batch(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const int32_t *pos_dev,
+                         const int32_t *rope_pos_dev, const float *k_rows, const float *v_rows, const float *q,
+                         float *q_out, uint64_t n_head, uint64_t q_stride) {
+    if (!kv) return fail(nullptr, "null kvq");
+    if (!kv->ctx) return fail(nullptr, kKvqClosed);
+    return guarded(kv->ctx, [&] {
+        return append(kv, {layer, seq0, 0, n_seq, 0, true, pos_dev, rope_pos_dev, k_rows, v_rows, q, q_out, n_head, q_stride}, q_out);
+    });
+}
+
+int zwg_kvq_rows_dev(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq,
+                     const int32_t *pos_dev, uint64_t pos0, uint64_t n, float *k_out, float *v_out) {
+    if (!kv) return fail(nullptr, "null kvq");
+    if (!kv->ctx) return fail(nullptr, kKvqClosed);
+    return guarded(kv->ctx, [&] { return rows(kv, layer0, n_layer, seq0, n_seq, pos_dev, pos0, n, k_out, v_out); });
+}
+
+int zwg_kvq_evict_dev(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq,
+                      const zwg_kvq_cut *cut, const float *weights, float *weights_out) {
+    if (!kv) return fail(nullptr, "null kvq");
+    if (!kv->ctx) return fail(nullptr, kKvqClosed);
+    if (!cut) return fail(kv->ctx, "null cut");
+    return guarded(kv->ctx, [&] { return evict(kv, layer0, n_layer, seq0, n_seq, cut, weights, weights_out); });
+}
+
+} // extern "C"

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -64,6 +65,20 @@ namespace zwg_host {
 // Record `msg` as the last error (of ctx, and of this thread) and return ZWG_ERROR.
 int fail(zwg_ctx *ctx, const std::string &msg);
 int fail_hip(zwg_ctx *ctx, const char *what, hipError_t e);
+// f() with any C++ exception it throws (an allocation that fails) turned into an error: none may cross the C ABI.
+template <class F> int guarded(zwg_ctx *ctx, F f) noexcept {
+    try {
+        return f();
+    } catch (const std::exception &x) {
+        try {
+            return fail(ctx, x.what());
+        } catch (...) {
+            return ZWG_ERROR;
+        }
+    } catch (...) {
+        return ZWG_ERROR;
+    }
+}
 // Grow staging buffer i of ctx to at least `bytes` (synchronises the stream when it grows).
 int ensure_stage(zwg_ctx *ctx, int i, uint64_t bytes);
 // Copy n_rows rows of `cols` floats, `stride` floats apart, from device `src` to host `dst` (same

@@ -488,6 +488,232 @@ class KVCache:
         return k, v
 
 
+class _Handle:
+    """An object made from a context: closed by close(), the context manager, or with the context."""
+
+    _destroy = ""  # the library's destroy function
+
+    def _own(self, ctx: Context, h: ctypes.c_void_p) -> None:
+        self.ctx, self._L, self._h = ctx, ctx._L, h
+        ctx._adopt(self)
+
+    @property
+    def handle(self):
+        if not self._h:
+            raise ZwgError(f"the {type(self).__name__} is closed")
+        return self._h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            getattr(self._L, self._destroy)(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _ptr(self, t, name: str, numel: int, dtype: str = "float32") -> int:
+        """Address of a contiguous CUDA tensor on the context's device of at least `numel` elements; 0 for None."""
+        import torch
+
+        if t is None:
+            return 0
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != getattr(torch, dtype):
+            raise ZwgError(f"{name} must be a CUDA {dtype} tensor")
+        if t.device.index != self.ctx.device:
+            raise ZwgError(f"{name} is on {t.device}, the context on device {self.ctx.device}")
+        if not t.is_contiguous():
+            raise ZwgError(f"{name} must be contiguous")
+        if t.numel() < numel:
+            raise ZwgError(f"{name} has {t.numel()} elements, the call needs {numel}")
+        return t.data_ptr()
+
+
+def _span(n_outer: int, outer: int, n: int, stride: int, row: int) -> int:
+    """Elements from the first to the last of n_outer x n rows of `row`, `outer` and `stride` apart."""
+    return (n_outer - 1) * outer + (n - 1) * stride + row if n_outer > 0 and n > 0 else 0
+
+
+def _count(name: str, *values) -> None:
+    for v in values:
+        if not isinstance(v, (int, np.integer)) or v < 0:
+            raise ZwgError(f"{name} must be a whole number, 0 or more")
+
+
+class Rope(_Handle):
+    """Rotary positions (zwg_rope_*): the rotation of src/llm.zig:221-238 over any rows of heads, in either pair
+    layout, over the first n_rot dims of a head (None: all of them) and with frequencies scaled for longer contexts.
+
+    layout: ROPE_HALF (pairs (j, j + n_rot/2)) or ROPE_INTERLEAVED (pairs (2j, 2j+1)); scaling: ROPE_NONE,
+    ROPE_LINEAR, ROPE_NTK or ROPE_YARN by `factor` (YaRN: over n_orig trained positions, between beta_slow and
+    beta_fast turns); mscale: factor on cos and sin (0: the method's own)."""
+
+    _destroy = "zwg_rope_destroy"
+
+    def __init__(self, ctx: Context, n_ctx: int, d: int, n_rot: Optional[int] = None, layout: int = _lib.ROPE_HALF,
+                 base: float = 1e6, scaling: int = _lib.ROPE_NONE, factor: float = 1.0, n_orig: int = 0,
+                 beta_fast: float = 0.0, beta_slow: float = 0.0, mscale: float = 0.0):
+        self._h = None
+        n_rot = d if n_rot is None else n_rot
+        _count("n_ctx, d, n_rot and n_orig", n_ctx, d, n_rot, n_orig)
+        self.desc = _lib.RopeDescC(n_ctx, d, n_rot, layout, scaling, base, factor, n_orig, beta_fast, beta_slow, mscale)
+        h = ctypes.c_void_p()
+        ctx._check(ctx._L.zwg_rope_create(ctx.handle, ctypes.byref(self.desc), ctypes.byref(h)))
+        self.n_ctx, self.d, self.n_rot = n_ctx, d, n_rot
+        self._own(ctx, h)
+
+    def apply(self, x, n: int, n_head: int, pos=0, out=None, x_stride: int = 0, out_stride: int = 0,
+              inverse: bool = False) -> None:
+        """Rotate n rows of n_head heads of x into out (None: in place): contiguous CUDA float32 tensors, rows
+        x_stride and out_stride floats apart (0: n_head * d).  pos: the first row's position (the next rows'
+        follow), or a CUDA int32 tensor of n positions (rows outside the tables are skipped).  inverse: by the
+        negative angles -- the gradient of the rotation and, with mscale 1, its inverse."""
+        import torch
+
+        _count("n, n_head, x_stride and out_stride", n, n_head, x_stride, out_stride)
+        row = n_head * self.d
+        xs = x_stride or row
+        os_ = out_stride or (xs if out is None else row)
+        xp = self._ptr(x, "x", _span(1, 0, n, xs, row))
+        op = xp if out is None else self._ptr(out, "out", _span(1, 0, n, os_, row))
+        pos0, pp = 0, 0
+        if isinstance(pos, torch.Tensor):
+            pp = self._ptr(pos, "pos", n, "int32")
+        else:
+            _count("pos", pos)
+            pos0 = pos
+        self.ctx._bind_torch_stream()
+        self.ctx._check(self._L.zwg_rope_apply_dev(self.handle, xp, n, n_head, xs, pp, pos0, op, os_,
+                                                   _lib.ROPE_INVERSE if inverse else 0))
+
+
+class KVQCache(_Handle):
+    """Key/value caches held in 8 bits (zwg_kvq_*): what KVCache is, at a quarter of the bytes, with one scale per
+    block of `block` tokens (16, 32 or 64) and KV head, for keys and for values.
+
+    fmt: KVQ_I8 (whole numbers, absmax / 127) or KVQ_E4M3 (8-bit floats, absmax / 448); rope: a Rope of head dim d
+    that rotates appended keys (and q), or None.  All tensors are contiguous CUDA tensors on the
+    context's device; every call is queued on torch's current stream."""
+
+    _destroy = "zwg_kvq_destroy"
+
+    def __init__(self, ctx: Context, n_layer: int, n_seq: int, n_ctx: int, n_head_kv: int, d: int, block: int = 32,
+                 fmt: int = _lib.KVQ_I8, rope: Optional[Rope] = None):
+        self._h = None
+        _count("n_layer, n_seq, n_ctx, n_head_kv, d and block", n_layer, n_seq, n_ctx, n_head_kv, d, block)
+        self.desc = _lib.KVQDescC(n_layer, n_seq, n_ctx, n_head_kv, d, block, fmt, 0)
+        h = ctypes.c_void_p()
+        ctx._check(ctx._L.zwg_kvq_create(ctx.handle, ctypes.byref(self.desc), rope.handle if rope is not None else None,
+                                         ctypes.byref(h)))
+        self.n_layer, self.n_seq, self.n_ctx, self.n_head_kv, self.d = n_layer, n_seq, n_ctx, n_head_kv, d
+        self.block, self.fmt, self.kvw = block, fmt, n_head_kv * d
+        self._own(ctx, h)
+
+    @property
+    def nbytes(self) -> int:
+        """Device bytes of the caches."""
+        return int(self._L.zwg_kvq_bytes(ctypes.byref(self.desc)))
+
+    def _queries(self, q, q_out, n: int, n_head: int, q_stride: int):
+        if q is None:
+            if q_out is not None:
+                raise ZwgError("q_out without q")
+            return 0, 0, 0
+        stride = q_stride or n_head * self.d
+        need = _span(1, 0, n, stride, n_head * self.d)
+        qp = self._ptr(q, "q", need)
+        return qp, qp if q_out is None else self._ptr(q_out, "q_out", need), stride
+
+    def append(self, layer: int, seq: int, pos: int, k_rows, v_rows, q=None, n_head: int = 0, q_stride: int = 0,
+               q_out=None, rope_pos: Optional[int] = None) -> None:
+        """Append k_rows.numel() / (n_head_kv * d) rows at pos.. of (layer, seq), keys (and q into q_out, or in
+        place) rotated at rope_pos.. (None: pos)."""
+        rope_pos = pos if rope_pos is None else rope_pos
+        _count("layer, seq, pos, rope_pos, n_head and q_stride", layer, seq, pos, rope_pos, n_head, q_stride)
+        n = k_rows.numel() // self.kvw
+        if n * self.kvw != k_rows.numel():
+            raise ZwgError("k_rows is not whole rows of n_head_kv * d")
+        kp, vp = self._ptr(k_rows, "k_rows", 0), self._ptr(v_rows, "v_rows", n * self.kvw)
+        qp, op, stride = self._queries(q, q_out, n, n_head, q_stride)
+        self.ctx._bind_torch_stream()
+        self.ctx._check(self._L.zwg_kvq_append(self.handle, layer, seq, pos, n, rope_pos, kp, vp, qp, op, n_head, stride))
+
+    def append_batch(self, layer: int, seq0: int, pos_dev, k_rows, v_rows, q=None, n_head: int = 0, q_stride: int = 0,
+                     q_out=None, rope_pos_dev=None) -> None:
+        """One row per sequence seq0.. at the positions in pos_dev (CUDA int32 tensor), rotated at those of
+        rope_pos_dev (None: pos_dev)."""
+        _count("layer, seq0, n_head and q_stride", layer, seq0, n_head, q_stride)
+        n = pos_dev.numel()
+        pp, rp = self._ptr(pos_dev, "pos_dev", 0, "int32"), self._ptr(rope_pos_dev, "rope_pos_dev", n, "int32")
+        kp, vp = self._ptr(k_rows, "k_rows", n * self.kvw), self._ptr(v_rows, "v_rows", n * self.kvw)
+        qp, op, stride = self._queries(q, q_out, n, n_head, q_stride)
+        self.ctx._bind_torch_stream()
+        self.ctx._check(self._L.zwg_kvq_append_batch(self.handle, layer, seq0, n, pp, rp, kp, vp, qp, op, n_head, stride))
+
+    def rows(self, layer0: int, n_layer: int, seq0: int, n_seq: int, n: int, k_out, v_out, pos=0) -> None:
+        """The values that n positions from pos (an int, or a CUDA int32 tensor, one per sequence) stand for, into
+        k_out and v_out [n_layer][n_seq][n][n_head_kv * d] (either may be None)."""
+        import torch
+
+        _count("layer0, n_layer, seq0, n_seq and n", layer0, n_layer, seq0, n_seq, n)
+        need = n_layer * n_seq * n * self.kvw
+        kp, vp = self._ptr(k_out, "k_out", need), self._ptr(v_out, "v_out", need)
+        pos0, pp = 0, 0
+        if isinstance(pos, torch.Tensor):
+            pp = self._ptr(pos, "pos", n_seq, "int32")
+        else:
+            _count("pos", pos)
+            pos0 = pos
+        self.ctx._bind_torch_stream()
+        self.ctx._check(self._L.zwg_kvq_rows_dev(self.handle, layer0, n_layer, seq0, n_seq, pp, pos0, n, kp, vp))
+
+    def attention(self, layer: int, seq0: int, n_seq: int, q, out, n_q: int, n_head: int, n_kv: int, causal: bool = True,
+                  n_kv_dev=None, weights=None, decay: float = 1.0, q_stride: int = 0, out_stride: int = 0,
+                  q_bstride: int = 0, out_bstride: int = 0, weights_stride: int = 0, weights_bstride: int = 0) -> None:
+        """softmax(q k^T / sqrt(d)) v over the first n_kv keys of sequences seq0.. (n_kv_dev: a CUDA int32 tensor of
+        each sequence's keys, n_kv then the most): q, out [n_seq][n_q][n_head * d], or at the given strides.  causal:
+        query i sees keys j <= n_kv - n_q + i.  weights [n_seq][n_head_kv][n_kv]: decay * weights + the sum of each
+        key's probabilities over the queries and the heads that share its KV head."""
+        _count("the sizes and strides", layer, seq0, n_seq, n_q, n_head, n_kv, q_stride, out_stride, q_bstride, out_bstride,
+               weights_stride, weights_bstride)
+        row = n_head * self.d
+        qs, os_ = q_stride or row, out_stride or row
+        qb, ob = q_bstride or n_q * qs, out_bstride or n_q * os_
+        ws = weights_stride or n_kv
+        wb = weights_bstride or self.n_head_kv * ws
+        qp = self._ptr(q, "q", _span(n_seq, qb, n_q, qs, row))
+        op = self._ptr(out, "out", _span(n_seq, ob, n_q, os_, row))
+        wp = self._ptr(weights, "weights", _span(n_seq, wb, self.n_head_kv, ws, n_kv))
+        c = _lib.KVQAttnC(n_q, n_kv, n_head, qs, os_, qb, ob, ws, wb, self._ptr(n_kv_dev, "n_kv_dev", n_seq, "int32"), decay,
+                          1 if causal else 0)
+        self.ctx._bind_torch_stream()
+        self.ctx._check(self._L.zwg_kvq_attention_dev(self.handle, layer, seq0, n_seq, qp, ctypes.byref(c), op, wp))
+
+    def evict(self, layer0: int, n_layer: int, seq0: int, n_seq: int, n_kv: int, n_keep: int, weights, weights_out=None,
+              n_first: int = 0, n_recent: int = 0, n_kv_dev=None, n_kv_out=None, kept=None, weights_stride: int = 0) -> None:
+        """Cut sequences of more than n_keep tokens to their first n_first, their last n_recent and the heaviest of
+        the rest, in order, per KV head.  weights (and weights_out, which may be the same tensor)
+        [n_layer][n_seq][n_head_kv][weights_stride, 0: n_kv]; kept: int32 [n_layer][n_seq][n_head_kv][n_keep]; n_kv_dev,
+        n_kv_out (may be the same): int32 [n_seq]."""
+        _count("the sizes", layer0, n_layer, seq0, n_seq, n_kv, n_keep, n_first, n_recent, weights_stride)
+        ws = weights_stride or n_kv
+        units = n_layer * n_seq * self.n_head_kv
+        need = _span(1, 0, units, ws, n_kv)
+        wp, wo = self._ptr(weights, "weights", need), self._ptr(weights_out, "weights_out", need)
+        c = _lib.KVQCutC(n_kv, n_keep, n_first, n_recent, ws, self._ptr(n_kv_dev, "n_kv_dev", n_seq, "int32"),
+                         self._ptr(n_kv_out, "n_kv_out", n_seq, "int32"), self._ptr(kept, "kept", units * n_keep, "int32"))
+        self.ctx._bind_torch_stream()
+        self.ctx._check(self._L.zwg_kvq_evict_dev(self.handle, layer0, n_layer, seq0, n_seq, ctypes.byref(c), wp, wo))
+
+
 class Decoder:
     """The Whisper text decoder on the device (zwg_decoder_*), src/decoder.zig's Decoder for n_windows
     windows decoded in lockstep: set_audio is Decoder.setAudio (src/decoder.zig:151-159) for a range
