@@ -37,10 +37,15 @@ static void layout() {
                     const int64_t a = zwg::kvq_at(is_v, t, c, d);
                     CHECK(a >= 0 && a < 192 * d, "byte %lld", (long long)a);
                     if (a >= 0 && a < 192 * d) ++hit[a];
-                    // a lane group's 16 bytes of a value tile: score tile q's keys 4 g .. 4 g + 3, q = 0 .. 3
+                    // what the lanes of a wave expect at 16 bytes each
+                    const int kb = (int)(a / 1024), l = (int)(a % 1024) / 64, g = (int)(a % 64) / 16, e = (int)(a % 16);
                     if (is_v) {
-                        const int s = zwg::kvq_v_slot(t & 63), g = s / 16, q = s / 4 % 4, i = s % 4;
-                        CHECK(16 * q + 4 * g + i == (t & 63), "slot of token %d", t);
+                        CHECK(t == 32 * (kb / (d / 32)) + 16 * (e / 4 % 2) + 4 * g + e % 4, "token %d", t);
+                        CHECK(c == 32 * (kb % (d / 32)) + 16 * (e / 8) + l, "dim %d", c);
+                    } else if (d == 32) {
+                        CHECK(t == 32 * kb + 16 * (e / 8) + l && c == 8 * g + e % 8, "token %d dim %d", t, c);
+                    } else {
+                        CHECK(t == 16 * (kb / (d / 64)) + l && c == 64 * (kb % (d / 64)) + 16 * g + e, "token %d dim %d", t, c);
                     }
                 }
             for (int h : hit) CHECK(h == 1, "a byte is used %d times", h);

@@ -11,9 +11,9 @@
 //
 // Layout of a product (v_mfma_f32_16x16x32_f16: A 16 x 32, B 32 x 16): keys or value dims are the rows of A, query
 // rows the columns of B.  Lane l holds A's row l % 16, B's column l % 16, both at contraction indices
-// 8 (l / 16) .. + 7, and of the result rows 4 (l / 16) .. + 3 of column l % 16.  A lane's 16 bytes of a key row are
-// two A operands; its scores (column l % 16, keys 16 q + 4 (l / 16) + i) are the B operand of the value product for
-// values stored in that order of keys (kvq_v_slot), so probabilities never leave the lane that made them.
+// 8 (l / 16) .. + 7, and of the result rows 4 (l / 16) .. + 3 of column l % 16.  A lane's 16 bytes of keys or values are
+// two A operands (kvq_at); its scores (column l % 16, keys 16 q + 4 (l / 16) + i) are the B operand of the value product
+// for values stored in that order of keys, so probabilities never leave the lane that made them.
 //
 // Few query rows (up to 8 share a KV head: a decode step): the 16 columns are 8 rows' hi terms and the same rows' lo
 // terms, and one product gives both.  More rows: 32 to a wave in two tiles, hi and lo as products of their own.
@@ -21,8 +21,11 @@
 // The maximum is a lazy one: a column's reference rises only when some score passes it by kSlack = 8 (log2 units),
 // so most tiles need no exchange between lanes and no rescaling.
 //
-// A workgroup's four waves take every fourth tile of 64 keys of one chunk and merge in LDS; chunks of one row
-// are merged by kvq_merge_kernel in their order.
+// A workgroup's four waves take every fourth tile of 32 keys of one chunk and merge in LDS; chunks of one row
+// are merged by kvq_merge_kernel.  Per wave and step 2 d / 32 KB are under way: the next step's keys are loaded once this
+// step's scores are formed, its values once this step's are added, into the same registers, so that four waves fit a
+// SIMD.  Bound by the reads and, in short calls, by the latency before the first product: 64 sequences of 1 .. 4096 keys
+// (d = 128, two KV heads, 67 MB) take 14.4 us, 4.7 TB/s, where a large copy moves 4.8.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -47,8 +50,24 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = zwg::kKvqTile; // keys of a wave's step
 constexpr int kWaves = zwg_planner::kKvqWaves;
 constexpr int kSplitTile = zwg_planner::kKvqSplitTile;
+constexpr int kCompactSeqs = 1024; // sequences whose key counts a workgroup goes through to find its work
+constexpr int kManyChunks = 32;
 constexpr float kSlack = 8.0f;
 constexpr float kProbScale = 64.0f; // 2^6: p * (sv / ref) * 2^6 <= 2^8 * 2 * 2^6
+
+// Division of n < 2^31 by a divisor known on the host: the kernels' first instructions are a good part of a short
+// call (they come from a cold instruction cache), and a general division is about 35 of them.
+struct Div {
+    uint32_t d, mul, shift;
+    Div() = default;
+    explicit Div(uint32_t x) : d(x), mul(0), shift(0) {
+        if (x <= 1) return;
+        uint32_t l = 32 - (uint32_t)__builtin_clz(x - 1); // ceil(log2 x)
+        mul = (uint32_t)(((1ull << (31 + l)) + x - 1) / x);
+        shift = l - 1;
+    }
+    __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+};
 
 struct KvqArgs {
     KvqView view;
@@ -61,7 +80,10 @@ struct KvqArgs {
     int32_t row_blocks;
     int32_t causal;
     float scale_log2;
-    int32_t chunk_len, max_chunks;
+    int32_t tau, max_chunks; // split tiles of a chunk aimed at
+    Div by_group, by_heads, by_per, by_seqs, by_tau, by_rows; // n_head_kv; n_head_kv * row_blocks; ...
+    int32_t per;
+    int32_t block_shift; // log2 of the tokens of a scale
     float *part_o;  // [row][max_chunks][d]
     float *part_ml; // [row][max_chunks][2]
     float *row_ml;  // [row][2]: the rows' final maximum and sum, for the weights; or nullptr
@@ -78,11 +100,25 @@ __device__ __forceinline__ int item_kv(const KvqArgs &a, int item) {
 }
 // Keys that row r of a (sequence, KV head) sees.
 __device__ __forceinline__ int row_limit(const KvqArgs &a, int n_kv, int r) {
-    return a.causal ? max(0, n_kv - a.n_q + r / a.group + 1) : n_kv;
+    return a.causal ? max(0, n_kv - a.n_q + a.by_group.of(r) + 1) : n_kv;
 }
 // Keys that the last row of row block rb sees.
 __device__ __forceinline__ int block_limit(const KvqArgs &a, int n_kv, int rb, int RB) {
     return row_limit(a, n_kv, min(a.rows, (rb + 1) * RB) - 1);
+}
+// a / b for 0 <= a < 2^22, 0 < b: the quotient of the floats is at most one off.
+__device__ __forceinline__ int div_small(int a, int b) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const int r = a - q * b;
+    return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+// zwg::unit_split with its divisions as above: the chunks of [0, kv_hi) and the keys of each.
+__device__ __forceinline__ int split(const KvqArgs &a, int kv_hi, int *chunk_keys) {
+    const int w = (kv_hi + kSplitTile - 1) / kSplitTile;
+    const int nc = min(max(a.by_tau.of(w + a.tau / 2), 1), a.max_chunks);
+    const int lt = max(1, div_small(w + nc - 1, nc));
+    *chunk_keys = lt * kSplitTile;
+    return max(1, div_small(w + lt - 1, lt));
 }
 // Row r of (item, KV head): partials and final statistics at this index.
 __device__ __forceinline__ int64_t row_at(const KvqArgs &a, int item, int hk, int r) {
@@ -153,27 +189,33 @@ template <int D, int CT, bool PACKED> struct Queries {
         return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
     }
 
-    __device__ __forceinline__ void load(const KvqArgs &a, int item, int hk, int r0, int lane) {
-        const int g = lane >> 4, col = lane & 15;
+    // a lane's elements as they are: the loads, which the caller issues before the codes' (they are needed first)
+    struct Raw {
+        f32x4 x[CT][G::kSteps][2];
+        __device__ __forceinline__ void load(const KvqArgs &a, int item, int hk, int r0, int lane) {
+            const int g = lane >> 4, col = lane & 15;
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                // rows behind the last repeat it: what they give is not stored
+                const int r = min(r0 + (PACKED ? (col & 7) : 16 * t + col), a.rows - 1);
+                const int qi = a.by_group.of(r);
+                const float *q = a.q + item * a.q_bstride + qi * a.q_stride + (int64_t)(hk * a.group + (r - qi * a.group)) * D;
+#pragma unroll
+                for (int s = 0; s < G::kSteps; ++s)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) x[t][s][h] = *reinterpret_cast<const f32x4 *>(q + at_dim(s, g) + 4 * h);
+            }
+        }
+    };
+
+    __device__ __forceinline__ void take(const KvqArgs &a, const Raw &raw, int lane) {
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-            const int r = r0 + (PACKED ? (col & 7) : 16 * t + col);
-            float x[G::kSteps][8];
             uint32_t top = 0;
-            const bool live = r < a.rows;
-            const int qi = live ? r / a.group : 0;
-            const float *q = a.q + item * a.q_bstride + qi * a.q_stride + (int64_t)(hk * a.group + (live ? r - qi * a.group : 0)) * D;
 #pragma unroll
             for (int s = 0; s < G::kSteps; ++s)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x4 v = live ? *reinterpret_cast<const f32x4 *>(q + at_dim(s, g) + 4 * h) : (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[s][4 * h + e] = v[e];
-                        top = max(top, abs_bits(v[e]));
-                    }
-                }
+                for (int k = 0; k < 8; ++k) top = max(top, abs_bits(raw.x[t][s][k >> 2][k & 3]));
             top = max(top, (uint32_t)__shfl_xor((int)top, 16));
             top = max(top, (uint32_t)__shfl_xor((int)top, 32));
             // largest element 1.m * 2^(e - 127) -> times 2^(141 - e): into 2^14 .. 2^15 (e 15 at least, so that
@@ -185,11 +227,11 @@ template <int D, int CT, bool PACKED> struct Queries {
             for (int s = 0; s < G::kSteps; ++s)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const float v = x[s][k] * up;
+                    const float v = raw.x[t][s][k >> 2][k & 3] * up;
                     const _Float16 hi = (_Float16)v;
                     const _Float16 lo = (_Float16)(v - (float)hi);
                     if (PACKED) {
-                        frag[t][0][s][k] = col < 8 ? hi : lo;
+                        frag[t][0][s][k] = (lane & 15) < 8 ? hi : lo;
                     } else {
                         frag[t][0][s][k] = hi;
                         frag[t][G::kParts - 1][s][k] = lo;
@@ -199,56 +241,242 @@ template <int D, int CT, bool PACKED> struct Queries {
     }
 };
 
-// 64 keys' codes: of the key tile q (16 keys) step s's operand.
-template <int D> struct KeyTile {
-    u32x4 w[4][D == 32 ? 1 : D / 64];
-    __device__ __forceinline__ void load(const uint8_t *keys, int lane) {
-        const int g = lane >> 4, row = lane & 15;
+constexpr int kQ = kTile / 16; // key tiles of a step
+
+// A unit's keys or values, range-checked by the hardware: a load past the end returns zeros and reads nothing, so loads
+// of steps that do not exist need no branch (a branch around loads makes the waits for earlier ones too long, as the
+// compiler must take the loads not to have been issued).
+constexpr uint32_t kNoStep = 0x80000000u;
+constexpr int kCachePolicyNT = 2; // read once a call: pass the caches without displacing lines
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t unit_codes(const uint8_t *codes, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(codes), 0, (int)bytes, 0x00020000);
+}
+
+// A step's keys or values: d / 32 KB, 16 bytes a lane each.
+template <int D> struct Codes {
+    u32x4 w[D / 32];
+    // at: the step's byte offset (its first key times d), or kNoStep; in the lane's offset, which is the checked one
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t codes, uint32_t at, int lane) {
+        const uint32_t off = at + 64u * (uint32_t)(lane & 15) + 16u * (uint32_t)(lane >> 4);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint8_t *p = keys + (16 * q + row) * D;
-            if (D == 32) {
-                const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p + 8 * g));
-                w[q][0] = (u32x4){v[0], v[1], 0u, 0u};
-            } else {
-#pragma unroll
-                for (int h = 0; h < (D == 32 ? 1 : D / 64); ++h)
-                    w[q][h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 64 * h + 16 * g));
-            }
-        }
+        for (int n = 0; n < D / 32; ++n)
+            w[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, (int)(off + 1024u * n), 0, kCachePolicyNT));
     }
-    __device__ __forceinline__ u32x2 step(int q, int s) const {
-        const u32x4 v = w[q][D == 32 ? 0 : s >> 1];
-        return s & 1 ? (u32x2){v[2], v[3]} : (u32x2){v[0], v[1]};
+    static __device__ __forceinline__ u32x2 half(u32x4 v, int h) { return h ? (u32x2){v[2], v[3]} : (u32x2){v[0], v[1]}; }
+    // key tile q's operand of score product st; value tile d's operand
+    __device__ __forceinline__ u32x2 key(int q, int st) const {
+        return D == 32 ? half(w[0], q) : half(w[q * (D / 64) + (st >> 1)], st & 1);
+    }
+    __device__ __forceinline__ u32x2 value(int d) const { return half(w[d >> 1], d & 1); }
+};
+// The scales of a step, one per 16 tokens (wave-uniform: scalar loads).
+struct Scales {
+    float s[kQ];
+    __device__ __forceinline__ void load(const float *scales, int k0, int shift) {
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) s[q] = scales[(k0 + 16 * q) >> shift];
     }
 };
 
-// The scores of 64 keys, log2 units, unmasked: column tile t, key tile q.
+// The products of a step's keys, unscaled: column tile t, key tile q.
 template <int D, int FMT, int CT, bool PACKED>
-__device__ __forceinline__ void score_tile(const Queries<D, CT, PACKED> &qs, const KeyTile<D> &kt, const float *ks, int block,
-                                           int k0, f32x4 (&s)[CT][4]) {
+__device__ __forceinline__ void score_tile(const Queries<D, CT, PACKED> &qs, const Codes<D> &kt, f32x4 (&s)[CT][kQ]) {
     using G = Geo<D, CT, PACKED>;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        f32x4 acc[CT];
+    for (int q = 0; q < kQ; ++q)
 #pragma unroll
-        for (int t = 0; t < CT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < CT; ++t) s[t][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < G::kSteps; ++st) {
-            const f16x8 k = codes_f16<FMT>(kt.step(q, st));
+    for (int st = 0; st < G::kSteps; ++st)
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            const f16x8 k = codes_f16<FMT>(kt.key(q, st));
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
                 for (int p = 0; p < G::kParts; ++p)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qs.frag[t][p][st], acc[t], 0, 0, 0);
+                    s[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qs.frag[t][p][st], s[t][q], 0, 0, 0);
         }
-        const float sk = ks[(k0 + 16 * q) / block];
+    if (PACKED) {
+#pragma unroll
+        for (int q = 0; q < kQ; ++q)
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][q][i] += other_half(s[t][q][i]);
+    }
+}
+
+// The running softmax of a wave's rows and the value products' operand.
+template <int D, int CT, bool PACKED> struct Softmax {
+    using G = Geo<D, CT, PACKED>;
+    float m[CT], l[CT], ref; // per column: reference maximum (log2 units) and this lane's sum; ref: see above
+    f32x4 o[CT][G::kDims];
+    f16x8 p[CT][G::kParts];
+
+    __device__ __forceinline__ void init() {
+        ref = 0.f;
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-            const float f = qs.back[t] * sk;
+            m[t] = -INFINITY;
+            l[t] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][q][i] = (PACKED ? acc[t][i] + other_half(acc[t][i]) : acc[t][i]) * f;
+            for (int d = 0; d < G::kDims; ++d) o[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
+    }
+
+    // Takes the products s of the keys from k0 on, of which column tile t sees those below lim[t] (k_end: the last
+    // limit of any row here; MASK: some column does not see them all), and forms p.
+    template <bool MASK>
+    __device__ __forceinline__ void take(const f32x4 (&s)[CT][kQ], const float (&back)[CT], const Scales &sk, const Scales &sv,
+                                         const int (&lim)[CT], int k0, int k_end, int lane) {
+        const int g = lane >> 4, col = lane & 15;
+        float top[CT];
+        bool rise = false;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            top[t] = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) {
+                float x = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!MASK || k0 + 16 * q + 4 * g + i < lim[t]) x = fmaxf(x, s[t][q][i]);
+                // scales are not negative: the largest product is the largest score (none seen: stays -infinity)
+                if (!MASK || x != -INFINITY) x *= back[t] * sk.s[q];
+                top[t] = fmaxf(top[t], x);
+            }
+            rise |= top[t] > m[t] + kSlack;
+        }
+        // the value scales relative to a power of two at most the largest met (NaNs aside); blocks behind the last
+        // visible key count for nothing, whatever they hold
+        float v[kQ], big = ref;
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            v[q] = !MASK || k0 + 16 * q < k_end ? sv.s[q] : 0.f;
+            big = fmaxf(big, v[q]);
+        }
+        const float ref_new = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, big) & 0x7f800000u);
+        if (__any(rise) || ref_new != ref) {
+            const float down = ref > 0.f ? ref * power_inverse(ref_new) : 1.f; // powers of two: exact
+            ref = ref_new;
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                const float m_new = fmaxf(m[t], groups_max(top[t]));
+                const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m[t] - m_new);
+                m[t] = m_new;
+                l[t] *= alpha;
+#pragma unroll
+                for (int d = 0; d < G::kDims; ++d) o[t][d] *= alpha * down;
+            }
+        }
+        const float inv_ref = ref > 0.f ? kProbScale * power_inverse(ref) : 0.f;
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) v[q] *= inv_ref;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const float mu = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) {
+                const float f = back[t] * sk.s[q];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float e = exp2_fast(__builtin_fmaf(s[t][q][i], f, -mu));
+                    float w = e * v[q];
+                    if (MASK && k0 + 16 * q + 4 * g + i >= lim[t]) e = w = 0.f; // its block's scales may be NaNs
+                    l[t] += e;
+                    const _Float16 h = (_Float16)w;
+                    const _Float16 r = (_Float16)(w - (float)h);
+                    const int k = 4 * q + i;
+                    if (PACKED) {
+                        p[t][0][k] = col < 8 ? h : r;
+                    } else {
+                        p[t][0][k] = h;
+                        p[t][G::kParts - 1][k] = r;
+                    }
+                }
+            }
+        }
+    }
+
+    // 1 / x of a power of two (normal, and its inverse too: scales lie between 2^-108 and 2^122)
+    static __device__ __forceinline__ float power_inverse(float x) {
+        return __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, x));
+    }
+
+    __device__ __forceinline__ void add(const f16x8 v, int d) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int q = 0; q < G::kParts; ++q) o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[t][q], o[t][d], 0, 0, 0);
+    }
+};
+
+// The work of workgroup `b`: over all (chunk, sequence, row block, KV head) with the chunk slowest, or, when the
+// sequences have their own key counts, over those with keys alone, sequence by sequence, so that consecutive
+// workgroups -- and so every CU -- get an even share however the counts differ.
+__device__ __forceinline__ bool find_unit(const KvqArgs &a, uint32_t b, int RB, int *item, int *rb, int *hk, int *chunk) {
+    const uint32_t per = (uint32_t)a.per;
+    uint32_t rest;
+    if (a.n_kv_dev && a.n_seq <= kCompactSeqs) {
+        const int lane = (int)(threadIdx.x & 63);
+        uint32_t base = 0;
+        bool hit = false;
+        for (int k = 0; k < a.n_seq && !hit; k += 64) {
+            const int it = k + lane;
+            uint32_t c = 0;
+            if (it < a.n_seq) {
+                int keys;
+                c = (uint32_t)split(a, block_limit(a, item_kv(a, it), a.row_blocks - 1, RB), &keys) * per;
+            }
+            uint32_t incl = c;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t v = (uint32_t)__shfl_up((int)incl, off);
+                if (lane >= off) incl += v;
+            }
+            const unsigned long long first = __ballot(base + incl > b);
+            if (first) {
+                const int f = __builtin_ctzll(first);
+                *item = k + f;
+                rest = b - (base + (uint32_t)__builtin_amdgcn_readlane((int)(incl - c), f));
+                hit = true;
+            } else {
+                base += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+            }
+        }
+        if (!hit) return false;
+        *chunk = a.by_per.of((int)rest);
+        rest -= (uint32_t)*chunk * per;
+    } else {
+        const int c = a.by_per.of((int)b);
+        rest = b - (uint32_t)c * per;
+        *chunk = a.by_seqs.of(c);
+        *item = c - *chunk * a.n_seq;
+    }
+    *rb = a.by_heads.of((int)rest);
+    *hk = (int)(rest - (uint32_t)*rb * (uint32_t)a.view.n_head_kv);
+    *item = __builtin_amdgcn_readfirstlane(*item);
+    *rb = __builtin_amdgcn_readfirstlane(*rb);
+    *hk = __builtin_amdgcn_readfirstlane(*hk);
+    *chunk = __builtin_amdgcn_readfirstlane(*chunk);
+    return true;
+}
+
+// A row's sums x (4 dims from c on) with maximum M and sum L: into out, or into its chunk's slot.
+template <int D>
+__device__ __forceinline__ void store_row(const KvqArgs &a, int item, int hk, int row, int c, int n_chunks, int chunk, float M,
+                                          float L, f32x4 x) {
+    const int64_t at = row_at(a, item, hk, row);
+    if (n_chunks == 1) {
+        const int qi = a.by_group.of(row), head = hk * a.group + row - qi * a.group;
+        const float inv = L != 0.f ? 1.f / L : 0.f; // a NaN stays one
+        *reinterpret_cast<f32x4 *>(a.out + item * a.out_bstride + qi * a.out_stride + (int64_t)head * D + c) = x * inv;
+        if (a.row_ml && c == 0) *reinterpret_cast<float2 *>(a.row_ml + 2 * at) = make_float2(M, L);
+    } else {
+        const int64_t slot = at * a.max_chunks + chunk;
+        *reinterpret_cast<f32x4 *>(a.part_o + slot * D + c) = x;
+        if (c == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * slot) = make_float2(M, L);
     }
 }
 
@@ -260,167 +488,87 @@ __global__ __launch_bounds__(64 * kWaves) void kvq_attn_kernel(KvqArgs a) {
     __shared__ float m_s[kWaves][RB], l_s[kWaves][RB];
 
     const KvqView &v = a.view;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, col = lane & 15;
-    // chunk slowest, so that the long sequences' work starts everywhere at once
-    int64_t b = blockIdx.x;
-    const int hk = (int)(b % v.n_head_kv);
-    b /= v.n_head_kv;
-    const int rb = (int)(b % a.row_blocks);
-    b /= a.row_blocks;
-    const int item = (int)(b % a.n_seq);
-    const int chunk = (int)(b / a.n_seq);
+    int item, rb, hk, chunk;
+    if (!find_unit(a, blockIdx.x, RB, &item, &rb, &hk, &chunk)) return;
 
     const int n_kv = item_kv(a, item);
     const int hi = block_limit(a, n_kv, rb, RB);
     int chunk_keys;
-    const int n_chunks = zwg::unit_split(hi, kSplitTile, a.chunk_len, a.max_chunks, &chunk_keys);
+    const int n_chunks = split(a, hi, &chunk_keys);
     if (chunk >= n_chunks) return;
     const int k_begin = chunk * chunk_keys, k_end = min(hi, k_begin + chunk_keys);
 
     const int64_t u = a.unit0 + (int64_t)item * v.n_head_kv + hk;
-    const uint8_t *keys = v.codes[0] + u * v.unit_bytes;
-    const uint8_t *vals = v.codes[1] + u * v.unit_bytes;
+    const __amdgpu_buffer_rsrc_t keys = unit_codes(v.codes[0] + u * v.unit_bytes, v.unit_bytes);
+    const __amdgpu_buffer_rsrc_t vals = unit_codes(v.codes[1] + u * v.unit_bytes, v.unit_bytes);
     const float *ks = v.scales[0] + u * v.n_blocks, *vs = v.scales[1] + u * v.n_blocks;
 
+    typename Queries<D, CT, PACKED>::Raw raw;
+    raw.load(a, item, hk, rb * RB, lane);
+    int k0 = k_begin + wave * kTile;
+    Codes<D> kt, vt;
+    Scales sk, sv;
+    kt.load(keys, k0 < k_end ? (uint32_t)k0 * D : kNoStep, lane);
+    vt.load(vals, k0 < k_end ? (uint32_t)k0 * D : kNoStep, lane);
+    sk.load(ks, k0 < k_end ? k0 : k_begin, a.block_shift);
+    sv.load(vs, k0 < k_end ? k0 : k_begin, a.block_shift);
     Queries<D, CT, PACKED> qs;
-    qs.load(a, item, hk, rb * RB, lane);
+    qs.take(a, raw, lane);
     int lim[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         const int r = rb * RB + (PACKED ? (col & 7) : 16 * t + col);
         lim[t] = r < a.rows ? min(k_end, row_limit(a, n_kv, r)) : 0;
     }
-    // the smallest limit of the block's rows: tiles below it need no mask (a block's rows behind the last have
-    // zero queries: what they compute is not stored)
+    // the smallest limit of the block's rows: tiles below it need no mask
     const int lim_all = min(k_end, row_limit(a, n_kv, rb * RB));
 
-    float m[CT], l[CT], ref = 0.f;
-    f32x4 o[CT][G::kDims];
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.f;
-#pragma unroll
-        for (int d = 0; d < G::kDims; ++d) o[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-
+    Softmax<D, CT, PACKED> sm;
+    sm.init();
 #pragma unroll 1
-    for (int k0 = k_begin + wave * kTile; k0 < k_end; k0 += kSplitTile) {
-        KeyTile<D> kt;
-        kt.load(keys + (int64_t)k0 * D, lane);
-        u32x4 vt[G::kDims];
+    while (k0 < k_end) {
+        f32x4 s[CT][kQ];
+        score_tile<D, FMT, CT, PACKED>(qs, kt, s);
+        // the next tile's keys on their way over this one's softmax and value products, its values over the next one's
+        // score products
+        const int next = k0 + kSplitTile;
+        const bool more = next < k_end;
+        const uint32_t at = more ? (uint32_t)next * D : kNoStep;
+        Scales sk_next, sv_next;
+        kt.load(keys, at, lane);
+        sk_next.load(ks, more ? next : k0, a.block_shift);
+        sv_next.load(vs, more ? next : k0, a.block_shift);
+        __builtin_amdgcn_sched_barrier(0);
+        // (few rows: one code for both, for the instruction cache's sake; the masks are a tenth of the work)
+        if (PACKED || k0 + kTile > lim_all)
+            sm.template take<true>(s, qs.back, sk, sv, lim, k0, k_end, lane);
+        else
+            sm.template take<false>(s, qs.back, sk, sv, lim, k0, k_end, lane);
 #pragma unroll
-        for (int d = 0; d < G::kDims; ++d)
-            vt[d] = __builtin_nontemporal_load(
-                reinterpret_cast<const u32x4 *>(vals + (int64_t)k0 * D + (16 * d + col) * 64 + 16 * g));
-        f32x4 s[CT][4];
-        score_tile<D, FMT, CT, PACKED>(qs, kt, ks, v.block, k0, s);
-        const bool mask = k0 + kTile > lim_all;
-        if (mask) {
-#pragma unroll
-            for (int t = 0; t < CT; ++t)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (k0 + 16 * q + 4 * g + i >= lim[t]) s[t][q][i] = -INFINITY;
-        }
-        // the reference maxima, raised when a score passes one by kSlack
-        float top[CT];
-        bool rise = false;
-#pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            top[t] = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[t] = fmaxf(top[t], s[t][q][i]);
-            rise |= top[t] > m[t] + kSlack;
-        }
-        if (__any(rise)) {
-#pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                const float m_new = fmaxf(m[t], groups_max(top[t]));
-                const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(m[t] - m_new);
-                m[t] = m_new;
-                l[t] *= alpha;
-#pragma unroll
-                for (int d = 0; d < G::kDims; ++d) o[t][d] *= alpha;
-            }
-        }
-        // the value scales relative to a power of two at most the largest met (NaNs aside)
-        float sv[4], big = ref;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            // blocks behind the last visible key count for nothing, whatever they hold
-            sv[q] = k0 + 16 * q < k_end ? vs[(k0 + 16 * q) / v.block] : 0.f;
-            big = fmaxf(big, sv[q]);
-        }
-        const float ref_new = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, big) & 0x7f800000u);
-        if (ref_new != ref) {
-            const float down = ref / ref_new; // powers of two: exact
-#pragma unroll
-            for (int t = 0; t < CT; ++t)
-#pragma unroll
-                for (int d = 0; d < G::kDims; ++d) o[t][d] *= down;
-            ref = ref_new;
-        }
-        const float inv_ref = ref > 0.f ? kProbScale / ref : 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sv[q] *= inv_ref;
-
-        f16x8 pf[CT][G::kParts][2];
-#pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            const float mu = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = exp2_fast(s[t][q][i] - mu);
-                    l[t] += p;
-                    float w = p * sv[q];
-                    // a masked key's block may have a NaN scale
-                    if (mask && k0 + 16 * q + 4 * g + i >= lim[t]) w = 0.f;
-                    const _Float16 h = (_Float16)w;
-                    const _Float16 r = (_Float16)(w - (float)h);
-                    const int j = q >> 1, e = 4 * (q & 1) + i;
-                    if (PACKED) {
-                        pf[t][0][j][e] = col < 8 ? h : r;
-                    } else {
-                        pf[t][0][j][e] = h;
-                        pf[t][G::kParts - 1][j][e] = r;
-                    }
-                }
-        }
-#pragma unroll
-        for (int d = 0; d < G::kDims; ++d)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const f16x8 vf = codes_f16<FMT>(j ? (u32x2){vt[d][2], vt[d][3]} : (u32x2){vt[d][0], vt[d][1]});
-#pragma unroll
-                for (int t = 0; t < CT; ++t)
-#pragma unroll
-                    for (int p = 0; p < G::kParts; ++p)
-                        o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t][p][j], o[t][d], 0, 0, 0);
-            }
+        for (int d = 0; d < G::kDims; ++d) sm.add(codes_f16<FMT>(vt.value(d)), d);
+        vt.load(vals, at, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        sk = sk_next;
+        sv = sv_next;
+        k0 = next;
     }
 
     // ---- the waves' results merged in LDS
-    const float unit = ref * (1.0f / kProbScale);
+    const float unit = sm.ref * (1.0f / kProbScale);
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        const float lt = groups_sum(l[t]);
+        const float lt = groups_sum(sm.l[t]);
         const int r = PACKED ? (col & 7) : 16 * t + col;
         const bool writes = !PACKED || col < 8;
         if (writes && g == 0) {
-            m_s[wave][r] = m[t];
+            m_s[wave][r] = sm.m[t];
             l_s[wave][r] = lt;
         }
 #pragma unroll
         for (int d = 0; d < G::kDims; ++d) {
-            f32x4 x = o[t][d];
+            f32x4 x = sm.o[t][d];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = (PACKED ? x[i] + other_half(x[i]) : x[i]) * unit;
             if (writes) *reinterpret_cast<f32x4 *>(&o_s[wave][r][16 * d + 4 * g]) = x;
@@ -436,69 +584,65 @@ __global__ __launch_bounds__(64 * kWaves) void kvq_attn_kernel(KvqArgs a) {
         for (int w = 0; w < kWaves; ++w) M = fmaxf(M, m_s[w][r]);
         float L = 0.f;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        if (M != -INFINITY) {
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float f = exp2_fast(m_s[w][r] - M); // 0 for a wave that saw no key of this row
-                L += f * l_s[w][r];
-                x += f * *reinterpret_cast<const f32x4 *>(&o_s[w][r][c]);
-            }
-        } else {
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) L += l_s[w][r]; // no key seen: 0; scores that are no numbers: NaN
+        for (int w = 0; w < kWaves; ++w) {
+            // 0 for a wave that saw no key of this row; with no key seen by any, sums of zeros, or of NaNs where the
+            // scores are no numbers
+            const float f = M == -INFINITY ? 1.f : exp2_fast(m_s[w][r] - M);
+            L += f * l_s[w][r];
+            x += f * *reinterpret_cast<const f32x4 *>(&o_s[w][r][c]);
         }
-        const int64_t at = row_at(a, item, hk, row);
-        if (n_chunks == 1) {
-            const int qi = row / a.group, head = hk * a.group + row - qi * a.group;
-            const float inv = L != 0.f ? 1.f / L : 0.f; // a NaN stays one
-            *reinterpret_cast<f32x4 *>(a.out + item * a.out_bstride + qi * a.out_stride + (int64_t)head * D + c) = x * inv;
-            if (a.row_ml && c == 0) {
-                a.row_ml[2 * at] = M;
-                a.row_ml[2 * at + 1] = L;
-            }
-        } else {
-            const int64_t slot = at * a.max_chunks + chunk;
-            *reinterpret_cast<f32x4 *>(a.part_o + slot * D + c) = x;
-            if (c == 0) {
-                a.part_ml[2 * slot] = M;
-                a.part_ml[2 * slot + 1] = L;
-            }
-        }
+        store_row<D>(a, item, hk, row, c, n_chunks, chunk, M, L, x);
     }
 }
 
-// The chunks of each row, in their order: a thread per (row, 4 dims).
-template <int D, int RB> __global__ __launch_bounds__(256) void kvq_merge_kernel(KvqArgs a, int64_t n_rows) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t at = i / (D / 4);
-    const int c = 4 * (int)(i % (D / 4));
-    if (at >= n_rows) return;
-    const int row = (int)(at % a.rows);
-    const int64_t ih = at / a.rows;
-    const int hk = (int)(ih % a.view.n_head_kv), item = (int)(ih / a.view.n_head_kv);
+// The chunks of each row, added in an order of their own: W dims of a row to a workgroup, W / 4 threads over them in
+// kGroups groups over the chunks, whose sums are added at the end.  W is d where the chunks are few; with many, a
+// narrow W brings more workgroups to a row (one CU takes in 30 to 40 GB/s).
+template <int D, int W, int RB> __global__ __launch_bounds__(256) void kvq_merge_kernel(KvqArgs a) {
+    constexpr int kGroups = 256 / (W / 4);
+    __shared__ __align__(16) f32x4 x_s[kGroups][W / 4];
+    __shared__ float red[4], l_s[kGroups];
+    const uint32_t at = blockIdx.x / (uint32_t)(D / W), first = blockIdx.x % (uint32_t)(D / W) * W;
+    const int ih = a.by_rows.of((int)at);
+    const int row = (int)at - ih * a.rows;
+    const int item = a.by_heads.of(ih), hk = ih - item * a.view.n_head_kv;
     int chunk_keys;
-    const int n_chunks = zwg::unit_split(block_limit(a, item_kv(a, item), row / RB, RB), kSplitTile, a.chunk_len, a.max_chunks, &chunk_keys);
+    const int n_chunks = split(a, block_limit(a, item_kv(a, item), row / RB, RB), &chunk_keys);
     if (n_chunks == 1) return; // written by the attention kernel
-    const float *ml = a.part_ml + 2 * at * a.max_chunks;
+    const int tid = threadIdx.x, grp = tid / (W / 4), c = tid % (W / 4);
+    const float *ml = a.part_ml + 2 * (int64_t)at * a.max_chunks;
+    const f32x4 *po = reinterpret_cast<const f32x4 *>(a.part_o + (int64_t)at * a.max_chunks * D + first) + c;
     float M = -INFINITY;
-    for (int k = 0; k < n_chunks; ++k) M = fmaxf(M, ml[2 * k]);
+    for (int k = tid; k < n_chunks; k += 256) M = fmaxf(M, ml[2 * k]);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+    if ((tid & 63) == 0) red[tid >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float L = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < n_chunks; ++k) {
+#pragma unroll 4
+    for (int k = grp; k < n_chunks; k += kGroups) {
         const float f = M == -INFINITY ? 1.f : exp2_fast(ml[2 * k] - M);
         L += f * ml[2 * k + 1];
-        x += f * *reinterpret_cast<const f32x4 *>(a.part_o + (at * a.max_chunks + k) * D + c);
+        x += f * po[(int64_t)k * (D / 4)];
     }
-    const int qi = row / a.group, head = hk * a.group + row - qi * a.group;
-    const float inv = L != 0.f ? 1.f / L : 0.f;
-    *reinterpret_cast<f32x4 *>(a.out + item * a.out_bstride + qi * a.out_stride + (int64_t)head * D + c) = x * inv;
-    if (a.row_ml && c == 0) {
-        a.row_ml[2 * at] = M;
-        a.row_ml[2 * at + 1] = L;
+    x_s[grp][c] = x;
+    if (c == 0) l_s[grp] = L;
+    __syncthreads();
+    if (tid >= W / 4) return;
+    L = 0.f;
+    x = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        L += l_s[k];
+        x += x_s[k][c];
     }
+    store_row<D>(a, item, hk, row, (int)first + 4 * c, 1, 0, M, L, x);
 }
 
-// Each key's probability summed over the rows that see it: a wave per 64 keys of a (sequence, KV head) goes over all
+// Each key's probability summed over the rows that see it: a wave per 32 keys of a (sequence, KV head) goes over all
 // row blocks in order, forms the scores again and adds exp2(s - M) / L in its lanes; the columns are added at the end.
 template <int D, int FMT, int CT, bool PACKED>
 __global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
@@ -511,19 +655,22 @@ __global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
     const int n_kv = item_kv(a, item);
     if (k0 >= n_kv) return;
     const int64_t u = a.unit0 + (int64_t)item * v.n_head_kv + hk;
-    KeyTile<D> kt;
-    kt.load(v.codes[0] + u * v.unit_bytes + (int64_t)k0 * D, lane);
-    const float *ks = v.scales[0] + u * v.n_blocks;
-    f32x4 acc[4];
+    Codes<D> kt;
+    kt.load(unit_codes(v.codes[0] + u * v.unit_bytes, v.unit_bytes), (uint32_t)k0 * D, lane);
+    Scales sk;
+    sk.load(v.scales[0] + u * v.n_blocks, k0, a.block_shift);
+    f32x4 acc[kQ];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < kQ; ++q) acc[q] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int rb = 0; rb < a.row_blocks; ++rb) {
         if (block_limit(a, n_kv, rb, RB) <= k0) continue;
+        typename Queries<D, CT, PACKED>::Raw raw;
+        raw.load(a, item, hk, rb * RB, lane);
         Queries<D, CT, PACKED> qs;
-        qs.load(a, item, hk, rb * RB, lane);
-        f32x4 s[CT][4];
-        score_tile<D, FMT, CT, PACKED>(qs, kt, ks, v.block, k0, s);
+        qs.take(a, raw, lane);
+        f32x4 s[CT][kQ];
+        score_tile<D, FMT, CT, PACKED>(qs, kt, s);
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const int r = rb * RB + (PACKED ? (col & 7) : 16 * t + col);
@@ -535,23 +682,24 @@ __global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
                 inv = ml[1] != 0.f ? 1.f / ml[1] : 0.f;
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < kQ; ++q)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (k0 + 16 * q + 4 * g + i < lim) acc[q][i] += exp2_fast(s[t][q][i] - M) * inv;
+                    if (k0 + 16 * q + 4 * g + i < lim)
+                        acc[q][i] += exp2_fast(__builtin_fmaf(s[t][q][i], qs.back[t] * sk.s[q], -M)) * inv;
         }
     }
     // over the 16 columns
     float *w = a.weights + item * a.w_bstride + hk * a.w_stride;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < kQ; ++q)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float x = acc[q][i];
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
             const int key = k0 + 16 * q + 4 * g + i;
-            // column 4 q + i of the group writes this key
+            // of the columns, all of which have the sum, 4 q + i writes this key
             if (col == 4 * q + i && key < n_kv) w[key] = (a.decay != 0.f ? a.decay * w[key] : 0.f) + x;
         }
 }
@@ -564,7 +712,10 @@ template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.max_chunks > 1) {
         const int64_t rows = (int64_t)a.n_seq * a.view.n_head_kv * a.rows;
-        kvq_merge_kernel<D, RB><<<(unsigned)((rows * (D / 4) + 255) / 256), 256, 0, stream>>>(a, rows);
+        if (a.max_chunks > kManyChunks)
+            kvq_merge_kernel<D, 16, RB><<<(unsigned)(rows * (D / 16)), 256, 0, stream>>>(a);
+        else
+            kvq_merge_kernel<D, D, RB><<<(unsigned)rows, 256, 0, stream>>>(a);
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.weights && a.n_kv > 0) {
@@ -616,8 +767,16 @@ int attention(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const 
     a.row_blocks = (int32_t)row_blocks;
     a.causal = (int32_t)s.causal;
     a.scale_log2 = (1.0f / std::sqrt((float)d.d)) * 1.4426950408889634f;
-    a.chunk_len = sp.chunk_len;
+    a.tau = sp.chunk_len / kSplitTile;
+    a.per = (int32_t)(d.n_head_kv * row_blocks);
+    a.by_group = Div((uint32_t)group);
+    a.by_heads = Div((uint32_t)d.n_head_kv);
+    a.by_per = Div((uint32_t)a.per);
+    a.by_seqs = Div((uint32_t)n_seq);
+    a.by_tau = Div((uint32_t)a.tau);
+    a.by_rows = Div((uint32_t)rows);
     a.max_chunks = sp.max_chunks;
+    a.block_shift = d.block == 16 ? 4 : d.block == 32 ? 5 : 6;
     a.row_ml = weights ? ctx->workspace : nullptr;
     a.part_ml = ctx->workspace + ws.part_ml;
     a.part_o = ctx->workspace + ws.part_o;

@@ -47,7 +47,7 @@ __device__ __forceinline__ void write_codes(uint8_t *codes, const float (*rows)[
         for (int i = threadIdx.x; i < (r1 - r0) * (D / 4); i += kAppendThreads) {
             const int r = r0 + i / (D / 4), c = 4 * (i % (D / 4));
             const float4 x = *reinterpret_cast<const float4 *>(&rows[r][c]);
-            *reinterpret_cast<uint32_t *>(codes + (first + r) * D + c) = zwg::kvq_encode4<FMT>(x.x, x.y, x.z, x.w, mul);
+            *reinterpret_cast<uint32_t *>(codes + zwg::kvq_at(0, first + r, c, D)) = zwg::kvq_encode4<FMT>(x.x, x.y, x.z, x.w, mul);
         }
     } else if (r0 == 0 && r1 == block_size) {
         for (int i = threadIdx.x; i < block_size / 4 * D; i += kAppendThreads) {
@@ -462,7 +462,7 @@ template <int D, int FMT> __global__ __launch_bounds__(kMoveThreads) void kvq_mo
                 float s = 0.0f;
                 if (t < a.n_keep) {
                     const int p = src[t];
-                    word = *reinterpret_cast<const uint32_t *>(codes + (int64_t)p * D + c);
+                    word = *reinterpret_cast<const uint32_t *>(codes + zwg::kvq_at(0, p, c, D));
                     s = scales[p / B];
                 }
                 x[k][0] = t < a.n_keep ? zwg::kvq_decode<FMT, 0>(word) * s : 0.0f;

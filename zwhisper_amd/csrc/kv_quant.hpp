@@ -3,10 +3,10 @@
 //
 // A unit is one (layer, sequence, KV head), u = (layer * n_seq + seq) * n_head_kv + head, of n_pad tokens (n_ctx
 // rounded up to 64).  Per unit:
-//   keys    [n_pad][d] bytes: a 16-byte piece of a row is a lane's operand of two matrix instructions
-//   values  [n_pad / 64][d][64] bytes: 64 tokens of one dim together, in the order of kvq_v_slot, in which
-//           the attention's probabilities lie in the lanes' registers after the score products, so that
-//           they feed the value products with no exchange between lanes
+//   keys    n_pad * d bytes, values the same, in the order of kvq_at: a wave's 64 lanes read 1 KB on end, 16 bytes a lane,
+//           and each half of these is an operand of a matrix instruction as it is; the values' order is the one in which
+//           the attention's probabilities lie in the lanes' registers after the score products, so that they
+//           feed the value products with no exchange between lanes
 //   scales  [n_pad / block] f32 each for keys and values
 //   the open block: its rows in f32 [block][d], keys and values, the block's index and filled rows, and
 //           each row's largest magnitude

@@ -22,15 +22,23 @@
 
 namespace zwg {
 
-constexpr int kKvqTile = 64; // tokens of a value tile, keys of a wave's step
+constexpr int kKvqTile = 32; // keys of a wave's step
+constexpr int kKvqPad = 64;  // a unit's tokens are padded to whole scale blocks of any size
 constexpr int kKvqMaxBlock = 64;
 
-// Byte of token t (0 .. 63) within its 64: token 16 q + 4 g + i is lane group g's i-th of score tile q.
-ZWG_KVQ_HD constexpr int kvq_v_slot(int t) { return ((t >> 2) & 3) * 16 + ((t >> 4) & 3) * 4 + (t & 3); }
-
-// Byte offset of (token, dim) in a unit's keys or values.
+// Byte offset of (token, dim) in a unit's keys or values: KBs that a wave's 64 lanes read together, 16 bytes a lane, two
+// operands of 8 codes each.  Lane 16 g + c reads, at 64 c + 16 g,
+//   keys    of 16 tokens and 64 dims (d 64 and 128): token c's dims 16 g .. 16 g + 15; at d = 32, of 32 tokens: dims
+//           8 g .. 8 g + 7 of tokens c and 16 + c
+//   values  of 32 tokens and 32 dims: dims c and 16 + c of tokens 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3 (the keys
+//           whose scores the lane holds after the score products)
 ZWG_KVQ_HD constexpr int64_t kvq_at(int is_v, int64_t token, int dim, int d) {
-    return is_v ? (token >> 6) * 64 * d + (int64_t)dim * 64 + kvq_v_slot((int)(token & 63)) : token * d + dim;
+    const int t = (int)(token & 31);
+    if (is_v)
+        return (token >> 5) * 32 * d + (dim >> 5) * 1024 + (dim & 15) * 64 + ((t >> 2) & 3) * 16 + ((dim >> 4) & 1) * 8 +
+               (t >> 4) * 4 + (t & 3);
+    if (d == 32) return (token >> 5) * 1024 + (dim >> 3) * 16 + (t & 15) * 64 + (t >> 4) * 8 + (dim & 7);
+    return (token >> 4) * 16 * d + (dim >> 6) * 1024 + (t & 15) * 64 + (dim & 63);
 }
 
 // What of an open block is held, keys and values each (they are written by different workgroups).
@@ -138,7 +146,7 @@ inline KvqLayout kvq_layout(const zwg_kvq_desc &d) {
     const auto up256 = [](uint64_t x) { return (x + 255) / 256 * 256; };
     KvqLayout l{};
     l.units = d.n_layer * d.n_seq * d.n_head_kv;
-    l.n_pad = (d.n_ctx + 63) / 64 * 64;
+    l.n_pad = (d.n_ctx + zwg::kKvqPad - 1) / zwg::kKvqPad * zwg::kKvqPad;
     l.codes = up256(l.units * l.n_pad * d.d);
     l.scales = up256(l.units * (l.n_pad / d.block) * sizeof(float));
     l.rows = up256(l.units * d.block * d.d * sizeof(float));
@@ -250,7 +258,7 @@ inline std::string check_kvq_attn(const zwg_kvq_desc &d, uint64_t layer, uint64_
         if (d.n_head_kv > 1 && s.weights_stride < s.n_kv) return "weights_stride is smaller than n_kv";
         if (n_seq > 1 && s.weights_bstride < (d.n_head_kv - 1) * s.weights_stride + s.n_kv)
             return "weights_bstride is smaller than a sequence's weights";
-        if ((s.n_kv + zwg::kKvqTile - 1) / zwg::kKvqTile > 65535) return "weights: n_kv must be below 2^22";
+        if ((s.n_kv + zwg::kKvqTile - 1) / zwg::kKvqTile > 65535) return "weights: n_kv must be below 2^21";
     }
     if (s.n_q * s.n_head * n_seq > 0x7fffffffull) return "n_q * n_head * sequences must be below 2^31";
     return "";
@@ -270,19 +278,25 @@ inline KvqWorkspace kvq_workspace(uint64_t rows, uint64_t chunks, uint64_t d, bo
     return w;
 }
 
-// Workgroups aimed at, four to a CU.
-constexpr uint64_t kKvqTargetBlocks = 1024;
-
 struct KvqSplit {
     int chunk_len, max_chunks;
 };
 
-// Keys of a chunk (unit_split's): units * chunks come near kKvqTargetBlocks, with at least one split tile to a chunk
-// and partials that fit the workspace.
+// Keys of a chunk (unit_split's), so that units * chunks come to about two workgroups a CU, or to four where chunks stay
+// at least kKvqLongChunk tiles long: each workgroup costs about 5 us before its first product and after its last, a tile
+// 0.9 us.  Measured, kernel and merge: 64 sequences of 1 .. 4096 keys, d = 128, 17.4 + 4.0 us at two a CU and 14.4 + 4.0 at
+// four (512 keys a chunk); one of 131,001 keys 13.3 + 5.5 at two (512 keys) and 15.2 + 7.6 at four (256 keys).
+// Partials have to fit the workspace.
+constexpr uint64_t kKvqLongChunk = 4;
+
 inline KvqSplit kvq_split(uint64_t units, uint64_t n_kv, uint64_t rows, uint64_t d, bool weights, uint64_t ws_bytes) {
     const uint64_t w = std::max<uint64_t>(1, (n_kv + kKvqSplitTile - 1) / kKvqSplitTile);
-    const uint64_t want = std::min<uint64_t>(w, std::max<uint64_t>(1, (kKvqTargetBlocks + units - 1) / units));
-    uint64_t tau = (w + want - 1) / want;
+    const auto tiles = [&](uint64_t blocks) {
+        const uint64_t want = std::min<uint64_t>(w, std::max<uint64_t>(1, (blocks + units - 1) / units));
+        return (w + want - 1) / want;
+    };
+    uint64_t tau = tiles(512);
+    if (tau > kKvqLongChunk) tau = std::max(kKvqLongChunk, tiles(1024));
     const auto bound = [&](uint64_t t) { return std::max<uint64_t>(1, (w + t / 2) / t); };
     while (bound(tau) > 1 && (bound(tau) > kKvqMaxChunks || kvq_workspace(rows, bound(tau), d, weights).total * sizeof(float) > ws_bytes))
         ++tau;
