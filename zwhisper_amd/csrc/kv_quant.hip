@@ -19,6 +19,9 @@ using zwg::KvqView;
 
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kAppendThreads = 256;
 constexpr int kPad = 4; // floats between the staged rows' ends and the next row: 16-byte rows on other banks
 
@@ -254,25 +257,56 @@ struct RowsArgs {
     float *out[2]; // [n_layer][n_seq][n][n_head_kv * d]
 };
 
-// Workgroups (x, y, z): 32 positions from 32 x of (layer, sequence) y; z: KV head and keys or values.
+// The i-th code of a lane's 16 bytes.
+template <int FMT> __device__ __forceinline__ float code_of(const u32x4 &w, int i) {
+    return zwg::kvq_decode_byte<FMT>((uint8_t)(w[i >> 2] >> (8 * (i & 3))));
+}
+
+// A wave per KB of codes of one unit's keys or values (32 positions have d / 32), read as the attention reads them: 16 bytes
+// a lane.  Workgroups (x, y, z): four such from 4 x on of (layer, sequence) y; z: KV head and keys or values.  Bound by its
+// stores, four times the bytes it reads.
 template <int D, int FMT> __global__ __launch_bounds__(256) void kvq_rows_kernel(RowsArgs a) {
     const KvqView &v = a.view;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
     const int is_v = blockIdx.z & 1, head = blockIdx.z >> 1;
     float *out = a.out[is_v];
     if (!out) return;
     const int64_t layer = a.layer0 + blockIdx.y / a.n_seq, i = blockIdx.y % a.n_seq;
     const int64_t u = (layer * v.n_seq + a.seq0 + i) * v.n_head_kv + head;
-    const uint8_t *codes = v.codes[is_v] + u * v.unit_bytes;
-    const float *scales = v.scales[is_v] + u * v.n_blocks;
     const int64_t start = a.pos_dev ? (int64_t)a.pos_dev[i] : a.pos0;
-    const int kvw = v.n_head_kv * D;
-    for (int k = threadIdx.x; k < 32 * D; k += 256) {
-        const int64_t t = (int64_t)blockIdx.x * 32 + k / D;
-        const int c = k % D;
-        const int64_t p = start + t;
-        if (t >= a.n || p < 0 || p >= v.n_ctx) continue;
-        out[((int64_t)blockIdx.y * a.n + t) * kvw + head * D + c] =
-            zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(is_v, p, c, D)]) * scales[p / v.block];
+    // the positions start .. start + n - 1 that the cache has, and this wave's tile of them
+    const int64_t lo = max(start, (int64_t)0), hi = min(start + a.n, (int64_t)v.n_ctx);
+    const int64_t kb = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t p0 = (lo / 32 + kb / (D / 32)) * 32;
+    const int n = (int)(kb % (D / 32));
+    if (p0 >= hi) return;
+    const uint8_t *codes = v.codes[is_v] + u * v.unit_bytes + p0 * D + 64 * col + 16 * g;
+    const float *scales = v.scales[is_v] + u * v.n_blocks;
+    const float s[2] = {scales[p0 / v.block], scales[(p0 + 16) / v.block]};
+    const int64_t kvw = (int64_t)v.n_head_kv * D;
+    out += ((int64_t)blockIdx.y * a.n - start) * kvw + head * D;
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(codes + 1024 * n);
+    if (is_v) {
+        // dims 32 n + col and 16 on, of tokens 16 q + 4 g + e
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int h = k >> 3, q = (k >> 2) & 1, e = k & 3;
+            const int64_t p = p0 + 16 * q + 4 * g + e;
+            if (p >= lo && p < hi) out[p * kvw + 32 * n + 16 * h + col] = code_of<FMT>(w, k) * s[q];
+        }
+    } else {
+        // dims 64 (n % (d / 64)) + 16 g .. of token 16 (n / (d / 64)) + col; at d = 32 dims 8 g .. of col and 16 + col
+        constexpr int kHalves = D == 128 ? 2 : 1;
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+            const int q = D == 32 ? k >> 3 : n / kHalves;
+            const int c = D == 32 ? 8 * g + (k & 7) : 64 * (n % kHalves) + 16 * g + k;
+            const int64_t p = p0 + 16 * q + col;
+            const float f = q ? s[1] : s[0];
+            if (p >= lo && p < hi)
+                *reinterpret_cast<float4 *>(out + p * kvw + c) = make_float4(code_of<FMT>(w, k) * f, code_of<FMT>(w, k + 1) * f,
+                                                                            code_of<FMT>(w, k + 2) * f, code_of<FMT>(w, k + 3) * f);
+        }
     }
 }
 
@@ -292,6 +326,8 @@ struct CutArgs {
     const float *w;
     float *w_out;
     int32_t *src;   // [unit of the call][n_keep]: the kept tokens' old positions
+    int32_t *dst;   // [unit of the call][n_kv rounded up to 32]: each token's new position, or -1
+    int64_t dst_stride;
     int32_t *count; // [unit of the call]: the tokens before the cut (the counts may be overwritten after it)
 };
 
@@ -317,7 +353,7 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
     const int n = a.n_kv_dev ? min(max(a.n_kv_dev[seq], 0), a.n_kv) : a.n_kv;
     const float *w = a.w + cu * a.w_stride;
     float *w_out = a.w_out ? a.w_out + cu * a.w_stride : nullptr;
-    int32_t *src = a.src + cu * a.n_keep;
+    int32_t *src = a.src + cu * a.n_keep, *dst = a.dst + cu * a.dst_stride;
     int32_t *kept = a.kept ? a.kept + cu * a.n_keep : nullptr;
     if (tid == 0) a.count[cu] = n;
     if (n <= a.n_keep) {
@@ -328,15 +364,26 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
         return;
     }
     const int lo = a.n_first, hi = n - a.n_recent; // the contested positions
+    // the first 8 of a thread's ranks stay in registers over the passes
+    constexpr int kHeld = 8;
+    uint32_t held[kHeld];
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+        const int i = lo + tid + k * kSelectThreads;
+        held[k] = i < hi ? rank_bits(w[i]) : 0u;
+    }
     uint32_t prefix = 0, left = (uint32_t)(a.n_keep - a.n_first - a.n_recent); // < hi - lo
 #pragma unroll 1
     for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
         if (tid < 256) hist[tid] = 0;
         __syncthreads();
-        for (int i = lo + tid; i < hi; i += kSelectThreads) {
-            const uint32_t r = rank_bits(w[i]);
+        const auto count = [&](uint32_t r) {
             if (shift == 24 || (r >> (shift + 8)) == prefix) atomicAdd(&hist[(r >> shift) & 255u], 1u);
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (lo + tid + k * kSelectThreads < hi) count(held[k]);
+        for (int i = lo + tid + kHeld * kSelectThreads; i < hi; i += kSelectThreads) count(rank_bits(w[i]));
         __syncthreads();
         if (wave == 0) {
             // the digit at which the counts from the top reach `left`: four digits a lane, lane 0 the highest
@@ -406,6 +453,7 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
         at += __popcll(sb & ((1ull << lane) - 1));
         // every weight of these positions is read (it decided `stays`, which the barrier above follows), and new
         // positions never lie above old ones: the weights may be compacted in place
+        if (i < (int)a.dst_stride) dst[i] = stays ? at : -1;
         if (stays) {
             src[at] = i;
             if (kept) kept[at] = i;
@@ -418,91 +466,208 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
 }
 
 constexpr int kMoveThreads = 1024;
+constexpr int kMoveWaves = kMoveThreads / 64;
 
-// One workgroup per (layer, sequence, head) and keys or values: new blocks in groups, in ascending order.  A
-// kept token never moves up, so the tokens of a group and all later ones lie at or above the group's first position:
-// once a group's codes are in registers (their magnitudes, which depend on them, are in LDS before the
-// barrier) its positions may be overwritten, and no later group misses what was there.
-template <int D, int FMT> __global__ __launch_bounds__(kMoveThreads) void kvq_move_kernel(CutArgs a) {
-    constexpr int kWords = 16;                         // words of four codes in a thread's registers
-    constexpr int kGroup = kMoveThreads * kWords * 4 / D; // tokens of a group: 2048 at d = 32 down to 512
+// One workgroup per (layer, sequence, head) and keys or values: new tokens in groups of kGroup, in ascending order.  A kept
+// token never moves up, so the tokens of a group and of all later ones lie at or above the group's first position: once a
+// group's codes are out of the cache (in registers, or in LDS; what a thread puts into LDS before the barrier depends on its
+// loads) its positions may be overwritten, and no later group misses what was there.
+//
+// Keys: a token's codes are runs of 16 bytes (8 at d = 32), gathered run by run.  Values: a token's codes lie one or two to a
+// 64-byte line, so the old tiles are read whole and in order, each wave one at a time, and their kept tokens' bytes are put into
+// LDS by new position, [d][kGroup].  Both are then taken as words of four codes twice: for the new blocks' largest
+// magnitudes, and for the new codes.
+template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_unit(const CutArgs &a, int64_t cu) {
+    constexpr int kGroup = 65536 / (D < 64 ? 64 : D); // 512 tokens at d = 128, else 1024
+    constexpr int kRow = kGroup + 16;                 // bytes of a dim's row in LDS: 4 words beyond a multiple of the banks
+    constexpr int kRun = D == 32 ? 8 : 16;            // bytes of a key run
+    constexpr int kRuns = kGroup * D / kRun / kMoveThreads; // runs of a thread: 4
     __shared__ uint32_t tops[kGroup / 16];
+    __shared__ float scale_s[kGroup];
+    __shared__ int32_t src_s[IS_V ? 1 : kGroup];
+    __shared__ __align__(16) uint8_t vals[IS_V ? D * kRow : 16];
     const KvqView &v = a.view;
-    const int tid = threadIdx.x;
-    const int64_t cu = blockIdx.x >> 1;
-    const int is_v = blockIdx.x & 1;
-    const int H = v.n_head_kv, B = v.block;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int H = v.n_head_kv;
+    const int shift = v.block == 16 ? 4 : v.block == 32 ? 5 : 6;
     const int64_t layer = a.layer0 + cu / ((int64_t)H * a.n_seq);
     const int64_t seq = (cu / H) % a.n_seq, head = cu % H;
     const int n = a.count[cu];
-    if (is_v && cu % H == 0 && cu / H < a.n_seq && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
+    if (IS_V && cu < (int64_t)H * a.n_seq && head == 0 && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
     if (n <= a.n_keep) return;
     const int64_t u = (layer * v.n_seq + a.seq0 + seq) * H + head;
-    uint8_t *codes = v.codes[is_v] + u * v.unit_bytes;
-    float *scales = v.scales[is_v] + u * v.n_blocks;
+    uint8_t *codes = v.codes[IS_V] + u * v.unit_bytes;
+    float *scales = v.scales[IS_V] + u * v.n_blocks;
     const int32_t *src = a.src + cu * a.n_keep;
-    if (tid == 0) v.open[2 * u + is_v].block = -1; // the open block's rows are others now
-    const int end = (a.n_keep + B - 1) / B * B;
+    const int32_t *dst = a.dst + cu * a.dst_stride;
+    if (tid == 0) v.open[2 * u + IS_V].block = -1; // the open block's rows are others now
+    const int end = ((a.n_keep + v.block - 1) >> shift) << shift;
 #pragma unroll 1
     for (int t0 = 0; t0 < end; t0 += kGroup) {
+        const int live = min(a.n_keep - t0, kGroup); // tokens of the group; the rest up to `end` becomes zeros
         if (tid < kGroup / 16) tops[tid] = 0;
-        __syncthreads();
-        // word k of a thread: keys: token t0 + w / (D / 4), dims 4 (w % (D / 4)) ..; values: dim w % D of tokens
-        // t0 + 4 (w / D) ..; w = k * threads + tid
-        float x[kWords][4];
+        for (int t = tid; t < kGroup; t += kMoveThreads) {
+            const int p = t < live ? src[t0 + t] : 0;
+            scale_s[t] = t < live ? scales[p >> shift] : 0.f;
+            if (!IS_V) src_s[t] = p;
+        }
+        u32x4 run[IS_V ? 1 : kRuns];
+        if (!IS_V) {
+            __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-            const int w = k * kMoveThreads + tid;
-            uint32_t top = 0;
-            int first;
-            if (!is_v) {
-                const int t = t0 + w / (D / 4), c = 4 * (w % (D / 4));
-                first = t;
-                uint32_t word = 0;
-                float s = 0.0f;
-                if (t < a.n_keep) {
-                    const int p = src[t];
-                    word = *reinterpret_cast<const uint32_t *>(codes + zwg::kvq_at(0, p, c, D));
-                    s = scales[p / B];
-                }
-                x[k][0] = t < a.n_keep ? zwg::kvq_decode<FMT, 0>(word) * s : 0.0f;
-                x[k][1] = t < a.n_keep ? zwg::kvq_decode<FMT, 1>(word) * s : 0.0f;
-                x[k][2] = t < a.n_keep ? zwg::kvq_decode<FMT, 2>(word) * s : 0.0f;
-                x[k][3] = t < a.n_keep ? zwg::kvq_decode<FMT, 3>(word) * s : 0.0f;
-            } else {
-                const int t = t0 + 4 * (w / D), c = w % D;
-                first = t;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[k][e] = 0.0f;
-                    if (t + e < a.n_keep) {
-                        const int p = src[t + e];
-                        x[k][e] = zwg::kvq_decode_byte<FMT>(codes[zwg::kvq_at(1, p, c, D)]) * scales[p / B];
+            for (int k = 0; k < kRuns; ++k) {
+                const int w = k * kMoveThreads + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
+                run[k] = (u32x4){0u, 0u, 0u, 0u};
+                if (t < live) {
+                    const uint8_t *at = codes + zwg::kvq_at(0, src_s[t], c, D);
+                    if (kRun == 16) {
+                        run[k] = *reinterpret_cast<const u32x4 *>(at);
+                    } else {
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                        run[k] = (u32x4){x[0], x[1], 0u, 0u};
                     }
                 }
             }
+            // a wave's 64 runs are of at most 16 aligned tokens: of one block
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, abs_bits(x[k][e]));
-            // a wave's 64 words are of at most 8 aligned tokens: of one block
+            for (int k = 0; k < kRuns; ++k) {
+                const int t = (k * kMoveThreads + tid) / (D / kRun);
+                // the largest code's value is the largest (one factor for all, and rounding keeps the order)
+                float m = 0.f;
 #pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
-            if ((tid & 63) == 0 && first < end) atomicMax(&tops[(first - t0) / B], top);
+                for (int i = 0; i < kRun; ++i) m = fmaxf(m, fabsf(code_of<FMT>(run[k], i)));
+                uint32_t top = t < live ? abs_bits(m * scale_s[t]) : 0u;
+#pragma unroll
+                for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+                if (lane == 0) atomicMax(&tops[t >> shift], top);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kRuns; ++k) {
+                const int w = k * kMoveThreads + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
+                if (t0 + t >= end) continue;
+                float scale, mul;
+                zwg::kvq_scale<FMT>(tops[t >> shift], &scale, &mul);
+                const float s = scale_s[t];
+                uint32_t word[kRun / 4];
+#pragma unroll
+                for (int i = 0; i < kRun / 4; ++i) {
+                    const bool on = t < live;
+                    word[i] = zwg::kvq_encode4<FMT>(on ? code_of<FMT>(run[k], 4 * i) * s : 0.f, on ? code_of<FMT>(run[k], 4 * i + 1) * s : 0.f,
+                                                    on ? code_of<FMT>(run[k], 4 * i + 2) * s : 0.f,
+                                                    on ? code_of<FMT>(run[k], 4 * i + 3) * s : 0.f, mul);
+                }
+                uint8_t *at = codes + zwg::kvq_at(0, t0 + t, c, D);
+                if (kRun == 16)
+                    *reinterpret_cast<u32x4 *>(at) = (u32x4){word[0], word[1], word[kRun / 4 - 2], word[kRun / 4 - 1]};
+                else
+                    *reinterpret_cast<u32x2 *>(at) = (u32x2){word[0], word[1]};
+                if (c == 0 && ((t0 + t) & (v.block - 1)) == 0) scales[(t0 + t) >> shift] = scale;
+            }
+        } else {
+            // the old tiles that hold the group's tokens
+            const int first = src[t0] >> 5, last = src[t0 + live - 1] >> 5;
+            const int g = lane >> 4, col = lane & 15;
+            for (int tile = first + wave; tile <= last; tile += kMoveWaves) {
+                int32_t to[8];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int4 x = *reinterpret_cast<const int4 *>(dst + 32 * tile + 16 * q + 4 * g);
+                    to[4 * q] = x.x - t0;
+                    to[4 * q + 1] = x.y - t0;
+                    to[4 * q + 2] = x.z - t0;
+                    to[4 * q + 3] = x.w - t0;
+                }
+                u32x4 w[D / 32];
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+                    w[k] = *reinterpret_cast<const u32x4 *>(codes + (int64_t)tile * 32 * D + 1024 * k + 64 * col + 16 * g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (to[e] >= 0 && to[e] < live) // -1, a token of another group: not here
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                vals[(32 * k + 16 * h + col) * kRow + to[e]] = (uint8_t)(w[k][2 * h + (e >> 2)] >> (8 * (e & 3)));
+            }
+            __syncthreads();
+            // new tiles, a wave to 32 tokens: lane (g, col) takes the 16 bytes of each KB that it would read there, from rows 4
+            // words (mod 64) apart at words g apart: all banks.  Word 2 h + q: dim 32 i + 16 h + col of tokens 16 q + 4 g ..
+            constexpr int kTiles = kGroup / 32 / kMoveWaves; // of a wave: 1 at d = 128, else 2
+            constexpr int kN = D / 32;
+            u32x4 code[kTiles][kN];
+#pragma unroll
+            for (int k = 0; k < kTiles; ++k) {
+                const int t = 32 * (k * kMoveWaves + wave);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int tq = t + 16 * q + 4 * g;
+                    float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < kN; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            code[k][i][2 * h + q] = *reinterpret_cast<const uint32_t *>(&vals[(32 * i + 16 * h + col) * kRow + tq]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(code_of<FMT>(code[k][i], 4 * (2 * h + q) + e)));
+                        }
+                    const float4 s = *reinterpret_cast<const float4 *>(&scale_s[tq]);
+                    uint32_t top = tq < live ? abs_bits(m[0] * s.x) : 0u;
+                    top = max(top, tq + 1 < live ? abs_bits(m[1] * s.y) : 0u);
+                    top = max(top, tq + 2 < live ? abs_bits(m[2] * s.z) : 0u);
+                    top = max(top, tq + 3 < live ? abs_bits(m[3] * s.w) : 0u);
+#pragma unroll
+                    for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+                    if (lane == 0) atomicMax(&tops[(t + 16 * q) >> shift], top);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kTiles; ++k) {
+                const int t = 32 * (k * kMoveWaves + wave);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int tq = t + 16 * q + 4 * g;
+                    float scale, mul;
+                    zwg::kvq_scale<FMT>(tops[(t + 16 * q) >> shift], &scale, &mul);
+                    if (lane == 0 && ((t + 16 * q) & (v.block - 1)) == 0 && t0 + t + 16 * q < end)
+                        scales[(t0 + t + 16 * q) >> shift] = scale;
+                    const float4 s4 = *reinterpret_cast<const float4 *>(&scale_s[tq]);
+                    const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                    for (int i = 0; i < kN; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                x[e] = tq + e < live ? code_of<FMT>(code[k][i], 4 * (2 * h + q) + e) * s[e] : 0.f;
+                            code[k][i][2 * h + q] = zwg::kvq_encode4<FMT>(x[0], x[1], x[2], x[3], mul);
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < kN; ++i) {
+                    // a last block of 16 may end in the middle of a tile: what lies behind it stays
+                    uint8_t *to = codes + (int64_t)(t0 + t) * D + 1024 * i + 64 * col + 16 * g;
+                    if (t0 + t + 16 < end) {
+                        *reinterpret_cast<u32x4 *>(to) = code[k][i];
+                    } else if (t0 + t < end) {
+                        *reinterpret_cast<uint32_t *>(to) = code[k][i][0];
+                        *reinterpret_cast<uint32_t *>(to + 8) = code[k][i][2];
+                    }
+                }
+            }
         }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-            const int w = k * kMoveThreads + tid;
-            const int t = is_v ? t0 + 4 * (w / D) : t0 + w / (D / 4);
-            if (t >= end) continue;
-            float scale, mul;
-            zwg::kvq_scale<FMT>(tops[(t - t0) / B], &scale, &mul);
-            const uint32_t word = zwg::kvq_encode4<FMT>(x[k][0], x[k][1], x[k][2], x[k][3], mul);
-            const int c = is_v ? w % D : 4 * (w % (D / 4));
-            *reinterpret_cast<uint32_t *>(codes + zwg::kvq_at(is_v, t, c, D)) = word;
-            if (c == 0 && t % B == 0) scales[t / B] = scale;
-        }
-        __syncthreads();
+        __syncthreads(); // the group's LDS is free, its codes written
     }
+}
+
+template <int D, int FMT> __global__ __launch_bounds__(kMoveThreads) void kvq_move_kernel(CutArgs a) {
+    if (blockIdx.x & 1)
+        move_unit<D, FMT, 1>(a, blockIdx.x >> 1);
+    else
+        move_unit<D, FMT, 0>(a, blockIdx.x >> 1);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -642,7 +807,9 @@ int rows(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t
     a.n_seq = (int32_t)n_seq;
     a.out[0] = k_out;
     a.out[1] = v_out;
-    const dim3 grid((unsigned)((n + 31) / 32), (unsigned)(n_layer * n_seq), (unsigned)(2 * d.n_head_kv));
+    // up to 31 positions of the first tile may lie before the first one asked for
+    const uint64_t kbs = (std::min(n, d.n_ctx) + 31 + 31) / 32 * (d.d / 32);
+    const dim3 grid((unsigned)((kbs + 3) / 4), (unsigned)(n_layer * n_seq), (unsigned)(2 * d.n_head_kv));
     ZWG_KVQ_DISPATCH(kvq_rows_kernel, d.d, d.format, <<<grid, 256, 0, ctx->stream>>>(a))
     e = hipGetLastError();
     return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "kvq rows launch", e);
@@ -681,7 +848,10 @@ int evict(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_
     a.w = weights;
     a.w_out = weights_out;
     a.count = reinterpret_cast<int32_t *>(ctx->workspace);
-    a.src = a.count + units;
+    // the new positions in rows of 16-byte multiples, which the kernel reads as such
+    a.dst_stride = (int64_t)kvq_cut_row(*c);
+    a.dst = a.count + (units + 3) / 4 * 4;
+    a.src = a.dst + (c->n_keep < c->n_kv ? units * kvq_cut_row(*c) : 0);
     kvq_select_kernel<<<(unsigned)units, kSelectThreads, 0, ctx->stream>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess) return fail_hip(ctx, "kvq select launch", e);

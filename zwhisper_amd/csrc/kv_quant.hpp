@@ -48,16 +48,18 @@ template <int FMT> __device__ __forceinline__ void kvq_scale(uint32_t top, float
 // Four codes in one word.  The products are at most Q (1 + 2^-23) in magnitude, which rounds to Q.  With a zero
 // multiplier every code is zero, whatever the element (an infinity times zero is no number).
 template <int FMT> __device__ __forceinline__ uint32_t kvq_encode4(float a, float b, float c, float e, float mul) {
+#pragma clang fp contract(off) // the product is rounded before the code is
     if (mul == 0.0f) return FMT == ZWG_KVQ_I8 ? 0x80808080u : 0u;
     a *= mul;
     b *= mul;
     c *= mul;
     e *= mul;
     if (FMT == ZWG_KVQ_I8) {
-        // rint rounds to even; +128 puts the codes into 1 .. 255
-        const uint32_t ua = (uint32_t)(int)(rintf(a) + 128.0f), ub = (uint32_t)(int)(rintf(b) + 128.0f);
-        const uint32_t uc = (uint32_t)(int)(rintf(c) + 128.0f), ue = (uint32_t)(int)(rintf(e) + 128.0f);
-        return ua | ub << 8 | uc << 16 | ue << 24;
+        // 3 * 2^22 + 128 + x: the sum is rounded to a whole number, ties to even, and its low byte is code + 128
+        constexpr float kWhole = 12582912.0f + 128.0f;
+        const uint32_t ua = __builtin_bit_cast(uint32_t, a + kWhole), ub = __builtin_bit_cast(uint32_t, b + kWhole);
+        const uint32_t uc = __builtin_bit_cast(uint32_t, c + kWhole), ue = __builtin_bit_cast(uint32_t, e + kWhole);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(ue, uc, 0x0c0c0400u), __builtin_amdgcn_perm(ub, ua, 0x0c0c0400u), 0x05040100u);
     }
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(c, e, w, true);

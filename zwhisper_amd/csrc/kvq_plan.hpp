@@ -221,9 +221,11 @@ inline std::string check_kvq_cut(const zwg_kvq_desc &d, uint64_t layer0, uint64_
     if (n_layer * n_seq * d.n_head_kv > 0x3fffffffull) return "too many (layer, sequence, head) units in one call";
     return "";
 }
-// The workspace of an eviction, bytes: each unit's tokens and kept positions.
+// The workspace of an eviction, bytes: each unit's tokens, their new positions (rows of whole tiles) and the kept ones' old
+// positions.
+inline uint64_t kvq_cut_row(const zwg_kvq_cut &c) { return (c.n_kv + 31) / 32 * 32; }
 inline uint64_t kvq_cut_bytes(uint64_t units, const zwg_kvq_cut &c) {
-    return (units + (c.n_keep < c.n_kv ? units * c.n_keep : 0)) * sizeof(int32_t);
+    return ((units + 3) / 4 * 4 + (c.n_keep < c.n_kv ? units * (c.n_keep + kvq_cut_row(c)) : 0)) * sizeof(int32_t);
 }
 
 // ---- attention over them
@@ -288,6 +290,7 @@ struct KvqSplit {
 // four (512 keys a chunk); one of 131,001 keys 13.3 + 5.5 at two (512 keys) and 15.2 + 7.6 at four (256 keys).
 // Partials have to fit the workspace.
 constexpr uint64_t kKvqLongChunk = 4;
+constexpr uint64_t kKvqUnsplit = 6;
 
 inline KvqSplit kvq_split(uint64_t units, uint64_t n_kv, uint64_t rows, uint64_t d, bool weights, uint64_t ws_bytes) {
     const uint64_t w = std::max<uint64_t>(1, (n_kv + kKvqSplitTile - 1) / kKvqSplitTile);
@@ -297,6 +300,7 @@ inline KvqSplit kvq_split(uint64_t units, uint64_t n_kv, uint64_t rows, uint64_t
     };
     uint64_t tau = tiles(512);
     if (tau > kKvqLongChunk) tau = std::max(kKvqLongChunk, tiles(1024));
+    if (w <= kKvqUnsplit) tau = w; // up to 6 steps a wave: less than a merge's launch
     const auto bound = [&](uint64_t t) { return std::max<uint64_t>(1, (w + t / 2) / t); };
     while (bound(tau) > 1 && (bound(tau) > kKvqMaxChunks || kvq_workspace(rows, bound(tau), d, weights).total * sizeof(float) > ws_bytes))
         ++tau;
