@@ -209,7 +209,7 @@ static void splits() {
         const uint64_t rows = units * (1 + rng() % RB), d = 32u << (rng() % 3);
         const bool weights = rng() % 2;
         const uint64_t ws = rng() % 4 ? 256ull << 20 : 1 + rng() % (1 << 20);
-        const KvqSplit s = kvq_split(units, n_kv, rows, d, weights, ws);
+        const KvqSplit s = kvq_split(units, n_kv, rows, d, weights, ws, it % 5 == 0);
         CHECK(s.chunk_len > 0 && s.chunk_len % kKvqSplitTile == 0 && s.max_chunks >= 1 && s.max_chunks <= (int)kKvqMaxChunks, "split");
         const KvqWorkspace w = kvq_workspace(rows, (uint64_t)s.max_chunks, d, weights);
         CHECK(s.max_chunks == 1 || w.total * 4 <= ws, "workspace %llu of %llu", (unsigned long long)w.total * 4, (unsigned long long)ws);

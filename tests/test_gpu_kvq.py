@@ -220,6 +220,9 @@ ATTEND = [  # lens, n_q, n_head, H, d, block, causal
     ([130], 130, 2, 1, 64, 32, True), ([257, 40, 33], 33, 6, 2, 128, 32, True), ([300], 9, 24, 2, 64, 64, False),
     ([1500], 5, 6, 6, 32, 32, False), ([40, 3], 9, 2, 1, 128, 16, True), ([1000], 40, 3, 1, 32, 16, True),
     ([2100], 1, 12, 2, 128, 64, True),
+    # calls of the prompt kernel: rows that fill no workgroup, sequences of unlike lengths, keys in many chunks
+    ([1500, 1490, 700], 560, 14, 2, 128, 32, True), ([3000], 1111, 6, 1, 64, 64, True), ([2900, 17], 700, 12, 2, 32, 16, False),
+    ([17000], 130, 2, 1, 128, 64, True),
 ]
 
 

@@ -113,9 +113,10 @@ __device__ __forceinline__ int div_small(int a, int b) {
     return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 // zwg::unit_split with its divisions as above: the chunks of [0, kv_hi) and the keys of each.
+__device__ __forceinline__ int split_bound(const KvqArgs &a, int w) { return min(max(a.by_tau.of(w + a.tau / 2), 1), a.max_chunks); }
 __device__ __forceinline__ int split(const KvqArgs &a, int kv_hi, int *chunk_keys) {
     const int w = (kv_hi + kSplitTile - 1) / kSplitTile;
-    const int nc = min(max(a.by_tau.of(w + a.tau / 2), 1), a.max_chunks);
+    const int nc = split_bound(a, w);
     const int lt = max(1, div_small(w + nc - 1, nc));
     *chunk_keys = lt * kSplitTile;
     return max(1, div_small(w + lt - 1, lt));
@@ -157,6 +158,10 @@ template <int FMT> __device__ __forceinline__ f16x8 codes_f16(u32x2 w) {
     return r;
 }
 
+// x of lane `lane`, the same for the whole wave.
+__device__ __forceinline__ float lane_value(float x, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
 // x of the lane 8 columns away (l ^ 8 within its row of 16).
 __device__ __forceinline__ float other_half(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
@@ -326,36 +331,53 @@ template <int D, int CT, bool PACKED> struct Softmax {
     }
 
     // Takes the products s of the keys from k0 on, of which column tile t sees those below lim[t] (k_end: the last
-    // limit of any row here; MASK: some column does not see them all), and forms p.
-    template <bool MASK>
-    __device__ __forceinline__ void take(const f32x4 (&s)[CT][kQ], const float (&back)[CT], const Scales &sk, const Scales &sv,
-                                         const int (&lim)[CT], int k0, int k_end, int lane) {
-        const int g = lane >> 4, col = lane & 15;
+    // limit of any row here; mask, the same in the whole wave: some column does not see them all): raises the references.
+    // f and w get what a product and a probability are to be multiplied by, and s is changed where the mask says so.  The
+    // branches are around few values: two copies of the whole would each want the accumulators in registers of their own.
+    __device__ __forceinline__ void prepare(f32x4 (&s)[CT][kQ], const float (&back)[CT], const Scales &sk, const Scales &sv,
+                                            const int (&lim)[CT], bool mask, int k0, int k_end, int lane, float (&f)[CT][kQ],
+                                            float (&w)[CT][kQ]) {
+        const int g = lane >> 4;
+        // blocks behind the last visible key count for nothing, whatever they hold
+        float big = ref;
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            const float v = k0 + 16 * q < k_end ? sv.s[q] : 0.f;
+            big = fmaxf(big, v);
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                f[t][q] = back[t] * sk.s[q];
+                w[t][q] = v;
+            }
+        }
+        if (mask) {
+            // an unseen key: -infinity; its block's scales may be zero or NaN, and are then not to be multiplied with
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int q = 0; q < kQ; ++q) {
+                    const bool sees = k0 + 16 * q < lim[t], zero = f[t][q] == 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = zero ? 0.f : s[t][q][i];
+                        s[t][q][i] = k0 + 16 * q + 4 * g + i < lim[t] ? x : -INFINITY;
+                    }
+                    if (zero || !sees) f[t][q] = 1.f;
+                    if (!sees) w[t][q] = 0.f;
+                }
+        }
+        // scales are not negative: the largest product is the largest score
         float top[CT];
         bool rise = false;
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             top[t] = -INFINITY;
 #pragma unroll
-            for (int q = 0; q < kQ; ++q) {
-                float x = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!MASK || k0 + 16 * q + 4 * g + i < lim[t]) x = fmaxf(x, s[t][q][i]);
-                // scales are not negative: the largest product is the largest score (none seen: stays -infinity)
-                if (!MASK || x != -INFINITY) x *= back[t] * sk.s[q];
-                top[t] = fmaxf(top[t], x);
-            }
+            for (int q = 0; q < kQ; ++q)
+                top[t] = fmaxf(top[t], fmaxf(fmaxf(s[t][q][0], s[t][q][1]), fmaxf(s[t][q][2], s[t][q][3])) * f[t][q]);
             rise |= top[t] > m[t] + kSlack;
         }
-        // the value scales relative to a power of two at most the largest met (NaNs aside); blocks behind the last
-        // visible key count for nothing, whatever they hold
-        float v[kQ], big = ref;
-#pragma unroll
-        for (int q = 0; q < kQ; ++q) {
-            v[q] = !MASK || k0 + 16 * q < k_end ? sv.s[q] : 0.f;
-            big = fmaxf(big, v[q]);
-        }
+        // the value scales relative to a power of two at most the largest met (NaNs aside)
         const float ref_new = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, big) & 0x7f800000u);
         if (__any(rise) || ref_new != ref) {
             const float down = ref > 0.f ? ref * power_inverse(ref_new) : 1.f; // powers of two: exact
@@ -372,30 +394,41 @@ template <int D, int CT, bool PACKED> struct Softmax {
         }
         const float inv_ref = ref > 0.f ? kProbScale * power_inverse(ref) : 0.f;
 #pragma unroll
-        for (int q = 0; q < kQ; ++q) v[q] *= inv_ref;
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) w[t][q] *= inv_ref;
+    }
+
+    // The probabilities of what prepare left, and p.  No branches: other products may go between.
+    __device__ __forceinline__ void weigh(const f32x4 (&s)[CT][kQ], const float (&f)[CT][kQ], const float (&w)[CT][kQ], int lane) {
+        const int col = lane & 15;
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const float mu = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
-            for (int q = 0; q < kQ; ++q) {
-                const float f = back[t] * sk.s[q];
+            for (int q = 0; q < kQ; ++q)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float e = exp2_fast(__builtin_fmaf(s[t][q][i], f, -mu));
-                    float w = e * v[q];
-                    if (MASK && k0 + 16 * q + 4 * g + i >= lim[t]) e = w = 0.f; // its block's scales may be NaNs
-                    l[t] += e;
-                    const _Float16 h = (_Float16)w;
-                    const _Float16 r = (_Float16)(w - (float)h);
+                for (int i = 0; i < 4; i += 2) {
+                    const float e0 = exp2_fast(__builtin_fmaf(s[t][q][i], f[t][q], -mu));
+                    const float e1 = exp2_fast(__builtin_fmaf(s[t][q][i + 1], f[t][q], -mu));
+                    l[t] += e0;
+                    l[t] += e1;
+                    const float x = e0 * w[t][q], y = e1 * w[t][q];
+                    // hi by truncation (two in one instruction); what is left fits 11 more bits, rounded
+                    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+                    const _Float16 hx = (_Float16)h[0], hy = (_Float16)h[1];
+                    const _Float16 rx = (_Float16)(x - (float)hx), ry = (_Float16)(y - (float)hy);
                     const int k = 4 * q + i;
                     if (PACKED) {
-                        p[t][0][k] = col < 8 ? h : r;
+                        p[t][0][k] = col < 8 ? hx : rx;
+                        p[t][0][k + 1] = col < 8 ? hy : ry;
                     } else {
-                        p[t][0][k] = h;
-                        p[t][G::kParts - 1][k] = r;
+                        p[t][0][k] = hx;
+                        p[t][0][k + 1] = hy;
+                        p[t][G::kParts - 1][k] = rx;
+                        p[t][G::kParts - 1][k + 1] = ry;
                     }
                 }
-            }
         }
     }
 
@@ -426,8 +459,11 @@ __device__ __forceinline__ bool find_unit(const KvqArgs &a, uint32_t b, int RB, 
             const int it = k + lane;
             uint32_t c = 0;
             if (it < a.n_seq) {
+                const int hi = block_limit(a, item_kv(a, it), a.row_blocks - 1, RB);
                 int keys;
-                c = (uint32_t)split(a, block_limit(a, item_kv(a, it), a.row_blocks - 1, RB), &keys) * per;
+                // fewer keys can be cut into more chunks (132 tiles into 44 of 3, 133 into 34 of 4), so with several row blocks
+                // the bound that grows with the keys
+                c = (uint32_t)(a.row_blocks == 1 ? split(a, hi, &keys) : split_bound(a, (hi + kSplitTile - 1) / kSplitTile)) * per;
             }
             uint32_t incl = c;
 #pragma unroll
@@ -541,11 +577,9 @@ __global__ __launch_bounds__(64 * kWaves) void kvq_attn_kernel(KvqArgs a) {
         sk_next.load(ks, more ? next : k0, a.block_shift);
         sv_next.load(vs, more ? next : k0, a.block_shift);
         __builtin_amdgcn_sched_barrier(0);
-        // (few rows: one code for both, for the instruction cache's sake; the masks are a tenth of the work)
-        if (PACKED || k0 + kTile > lim_all)
-            sm.template take<true>(s, qs.back, sk, sv, lim, k0, k_end, lane);
-        else
-            sm.template take<false>(s, qs.back, sk, sv, lim, k0, k_end, lane);
+        float f[CT][kQ], w[CT][kQ];
+        sm.prepare(s, qs.back, sk, sv, lim, k0 + kTile > lim_all, k0, k_end, lane, f, w);
+        sm.weigh(s, f, w, lane);
 #pragma unroll
         for (int d = 0; d < G::kDims; ++d) sm.add(codes_f16<FMT>(vt.value(d)), d);
         vt.load(vals, at, lane);
@@ -596,6 +630,133 @@ __global__ __launch_bounds__(64 * kWaves) void kvq_attn_kernel(KvqArgs a) {
     }
 }
 
+// Prompts: 128 rows of a (sequence, KV head) to a workgroup, 16 to each of 8 waves, over the same keys.  A step's codes are
+// read once, a KB a wave, turned into f16 operands and put into LDS, from where all waves feed their products (turning
+// codes into f16 takes a wave as many instructions as its softmax, so it is shared); the next step's are put into the other
+// half of LDS behind this step's products, and those of the one after that are on their way.
+//
+// Bound by the sum of matrix and vector instructions, which do not overlap here: 1024 queries of 12 heads over 8000 keys (d =
+// 128) take 123 us, of which the products alone, 94 GFLOP with their hi and lo terms, take 64 (1.47 PFLOP/s, what a large
+// library product reaches on this card) and everything else alone 55.  For that reason none of these measured faster: the next
+// step's score products between this step's softmax instructions (124 us), 32 rows to each of 4 waves (124), 64 keys between
+// two barriers (127).
+constexpr int kPromptRows = 128;
+constexpr int kPromptWaves = 8;
+
+template <int D, int FMT> __global__ __launch_bounds__(64 * kPromptWaves, 4) void kvq_prompt_kernel(KvqArgs a) {
+    constexpr int CT = 1;
+    using G = Geo<D, CT, false>;
+    constexpr int kKB = D / 32; // KBs of a step's keys, and of its values: at most one a wave
+    static_assert(2 * kKB <= kPromptWaves, "a KB a wave");
+    __shared__ __align__(16) f16x8 stage[2][4 * kKB][64]; // operands: [key tile][step] of keys, then value tiles
+    const KvqView &v = a.view;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, col = lane & 15;
+    int item, rb, hk, chunk;
+    if (!find_unit(a, blockIdx.x, kPromptRows, &item, &rb, &hk, &chunk)) return;
+    if (a.causal) rb = a.row_blocks - 1 - rb; // the longest first
+
+    const int n_kv = item_kv(a, item);
+    const int hi = block_limit(a, n_kv, rb, kPromptRows);
+    int chunk_keys;
+    const int n_chunks = split(a, hi, &chunk_keys);
+    if (chunk >= n_chunks) return;
+    const int k_begin = chunk * chunk_keys, k_end = min(hi, k_begin + chunk_keys);
+
+    const int64_t u = a.unit0 + (int64_t)item * v.n_head_kv + hk;
+    const int of_val = wave >= kKB; // this wave's KB is of the values
+    const __amdgpu_buffer_rsrc_t codes = unit_codes((of_val ? v.codes[1] : v.codes[0]) + u * v.unit_bytes, v.unit_bytes);
+    // A step's scales are vector loads of their own, a lane to a key tile, a step ahead: scalar loads beside the LDS reads
+    // would have the products wait for both.
+    const __amdgpu_buffer_rsrc_t scales[2] = {
+        unit_codes(reinterpret_cast<const uint8_t *>(v.scales[0] + u * v.n_blocks), (int64_t)v.n_blocks * 4),
+        unit_codes(reinterpret_cast<const uint8_t *>(v.scales[1] + u * v.n_blocks), (int64_t)v.n_blocks * 4)};
+
+    const int row0 = rb * kPromptRows + 16 * CT * wave;
+    typename Queries<D, CT, false>::Raw raw;
+    raw.load(a, item, hk, row0, lane);
+
+    u32x4 held;
+    uint32_t next_scale[2];
+    const auto load = [&](int k0) { // steps that do not exist read nothing and come out as zeros
+        const bool is = k0 < k_end;
+        const uint32_t scale_at = is ? 4u * ((uint32_t)(k0 + 16 * (lane & (kQ - 1))) >> a.block_shift) : kNoStep;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) next_scale[i] = __builtin_amdgcn_raw_buffer_load_b32(scales[i], (int)scale_at, 0, 0);
+        const uint32_t at = is && wave < 2 * kKB ? (uint32_t)k0 * D + 1024u * (uint32_t)(of_val ? wave - kKB : wave) : kNoStep;
+        held = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, (int)(at + 64u * col + 16u * g), 0, 0));
+    };
+    const auto put = [&](int half) {
+        if (wave >= 2 * kKB) return;
+        // a KB is two operands: of keys (d = 128) steps 2 (n % 2) and 2 (n % 2) + 1 of key tile n / 2; (64) both steps of tile n;
+        // (32) both key tiles' one step -- in every case 2 n and 2 n + 1 of [key tile][step] -- of values tiles 2 n and 2 n + 1
+        stage[half][2 * wave][lane] = codes_f16<FMT>((u32x2){held[0], held[1]});
+        stage[half][2 * wave + 1][lane] = codes_f16<FMT>((u32x2){held[2], held[3]});
+    };
+    Scales sk, sv; // of the step at hand
+    const auto take_scales = [&] {
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            sk.s[q] = lane_value(__builtin_bit_cast(float, next_scale[0]), q);
+            sv.s[q] = lane_value(__builtin_bit_cast(float, next_scale[1]), q);
+        }
+    };
+    load(k_begin);
+    Queries<D, CT, false> qs;
+    qs.take(a, raw, lane);
+    const int row = row0 + col;
+    const int lim[CT] = {row < a.rows ? min(k_end, row_limit(a, n_kv, row)) : 0};
+    // the smallest and the largest limit of this wave's rows
+    const int lim_all = row0 < a.rows ? min(k_end, row_limit(a, n_kv, row0)) : 0;
+    const int lim_any = row0 < a.rows ? min(k_end, row_limit(a, n_kv, min(a.rows, row0 + 16 * CT) - 1)) : 0;
+
+    Softmax<D, CT, false> sm;
+    sm.init();
+    put(0);
+    take_scales();
+    load(k_begin + kTile);
+    __syncthreads();
+    int half = 0;
+#pragma unroll 1
+    for (int k0 = k_begin; k0 < k_end; k0 += kTile) {
+        if (k0 < lim_any) {
+            f32x4 s[CT][kQ];
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) s[0][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < G::kSteps; ++st)
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int q = 0; q < kQ; ++q)
+                        s[0][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(stage[half][q * G::kSteps + st][lane], qs.frag[0][p][st], s[0][q], 0, 0, 0);
+            float f[CT][kQ], w[CT][kQ];
+            sm.prepare(s, qs.back, sk, sv, lim, k0 + kTile > lim_all, k0, k_end, lane, f, w);
+            sm.weigh(s, f, w, lane);
+            // two value tiles in turn: no product waits for the one before it
+#pragma unroll
+            for (int d = 0; d < G::kDims; d += 2)
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        sm.o[0][d + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(stage[half][2 * kKB + d + e][lane], sm.p[0][p], sm.o[0][d + e], 0, 0, 0);
+        }
+        // every wave left the other half at the last barrier
+        half ^= 1;
+        put(half);
+        take_scales();
+        load(k0 + 2 * kTile);
+        __syncthreads();
+    }
+
+    const float unit = sm.ref * (1.0f / kProbScale);
+    const float L = groups_sum(sm.l[0]);
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int d = 0; d < G::kDims; ++d) store_row<D>(a, item, hk, row, 16 * d + 4 * g, n_chunks, chunk, sm.m[0], L, sm.o[0][d] * unit);
+}
+
 // The chunks of each row, added in an order of their own: W dims of a row to a workgroup, W / 4 threads over them in
 // kGroups groups over the chunks, whose sums are added at the end.  W is d where the chunks are few; with many, a
 // narrow W brings more workgroups to a row (one CU takes in 30 to 40 GB/s).
@@ -642,92 +803,168 @@ template <int D, int W, int RB> __global__ __launch_bounds__(256) void kvq_merge
     store_row<D>(a, item, hk, row, (int)first + 4 * c, 1, 0, M, L, x);
 }
 
-// Each key's probability summed over the rows that see it: a wave per 32 keys of a (sequence, KV head) goes over all
-// row blocks in order, forms the scores again and adds exp2(s - M) / L in its lanes; the columns are added at the end.
-template <int D, int FMT, int CT, bool PACKED>
-__global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
+// The same for up to MAXC chunks: a thread per (row, 4 dims), all of its loads on their way at once (those of slots past
+// the row's chunks repeat the last).
+template <int D, int MAXC, int RB> __global__ __launch_bounds__(256) void kvq_merge_few_kernel(KvqArgs a, int n_rows) {
+    const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+    const int at = i / (D / 4), c = i % (D / 4);
+    if (at >= n_rows) return;
+    const int last = a.max_chunks - 1;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + (int64_t)at * a.max_chunks;
+    const f32x4 *po = reinterpret_cast<const f32x4 *>(a.part_o + (int64_t)at * a.max_chunks * D) + c;
+    float2 s[MAXC];
+    f32x4 x[MAXC];
+#pragma unroll
+    for (int k = 0; k < MAXC; ++k) {
+        s[k] = ml[min(k, last)];
+        x[k] = po[min(k, last) * (D / 4)];
+    }
+    const int ih = a.by_rows.of(at);
+    const int row = at - ih * a.rows;
+    const int item = a.by_heads.of(ih), hk = ih - item * a.view.n_head_kv;
+    int chunk_keys;
+    const int n_chunks = split(a, block_limit(a, item_kv(a, item), row / RB, RB), &chunk_keys);
+    if (n_chunks == 1) return; // written by the attention kernel
+    float M = -INFINITY, L = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < MAXC; ++k)
+        if (k < n_chunks) M = fmaxf(M, s[k].x);
+#pragma unroll
+    for (int k = 0; k < MAXC; ++k) {
+        if (k >= n_chunks) continue; // the slots of other calls may hold anything
+        const float f = M == -INFINITY ? 1.f : exp2_fast(s[k].x - M);
+        L += f * s[k].y;
+        sum += f * x[k];
+    }
+    store_row<D>(a, item, hk, row, 4 * c, 1, 0, M, L, sum);
+}
+
+// Each key's probability summed over the rows that see it: a wave per 128 keys of a (sequence, KV head) keeps their codes in
+// registers, goes over all row blocks in order, forms the scores again and adds exp2(s - M) / L in its lanes; the columns are
+// added at the end.  Turning a row block into operands costs about what scoring 32 keys does, so it is done for 128.
+constexpr int kWeightTiles = 4;
+constexpr int kWeightKeys = kWeightTiles * kTile;
+
+template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
+    constexpr int CT = 1;
     using G = Geo<D, CT, PACKED>;
     constexpr int RB = G::kRows;
     const KvqView &v = a.view;
     const int lane = threadIdx.x, g = lane >> 4, col = lane & 15;
-    const int hk = blockIdx.x % v.n_head_kv, item = blockIdx.x / v.n_head_kv;
-    const int k0 = blockIdx.y * kTile;
+    const int item = a.by_heads.of((int)blockIdx.x), hk = (int)blockIdx.x - item * v.n_head_kv;
+    const int k0 = blockIdx.y * kWeightKeys;
     const int n_kv = item_kv(a, item);
     if (k0 >= n_kv) return;
+    const int row_blocks = (a.rows + RB - 1) / RB;
+    // causal rows from here on see a key of this wave
+    int rb = 0;
+    while (rb < row_blocks - 1 && block_limit(a, n_kv, rb, RB) <= k0) ++rb;
+    typename Queries<D, CT, PACKED>::Raw raw;
+    raw.load(a, item, hk, rb * RB, lane);
     const int64_t u = a.unit0 + (int64_t)item * v.n_head_kv + hk;
-    Codes<D> kt;
-    kt.load(unit_codes(v.codes[0] + u * v.unit_bytes, v.unit_bytes), (uint32_t)k0 * D, lane);
-    Scales sk;
-    sk.load(v.scales[0] + u * v.n_blocks, k0, a.block_shift);
-    f32x4 acc[kQ];
+    const __amdgpu_buffer_rsrc_t keys = unit_codes(v.codes[0] + u * v.unit_bytes, v.unit_bytes);
+    Codes<D> kt[kWeightTiles];
+    Scales sk[kWeightTiles];
 #pragma unroll
-    for (int q = 0; q < kQ; ++q) acc[q] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < kWeightTiles; ++n) {
+        const int k = k0 + n * kTile;
+        kt[n].load(keys, k < n_kv ? (uint32_t)k * D : kNoStep, lane);
+        sk[n].load(v.scales[0] + u * v.n_blocks, k < n_kv ? k : k0, a.block_shift);
+    }
+    f32x4 acc[kWeightTiles][kQ];
+#pragma unroll
+    for (int n = 0; n < kWeightTiles; ++n)
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) acc[n][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int rb = 0; rb < a.row_blocks; ++rb) {
-        if (block_limit(a, n_kv, rb, RB) <= k0) continue;
-        typename Queries<D, CT, PACKED>::Raw raw;
-        raw.load(a, item, hk, rb * RB, lane);
+    for (; rb < row_blocks; ++rb) {
         Queries<D, CT, PACKED> qs;
         qs.take(a, raw, lane);
-        f32x4 s[CT][kQ];
-        score_tile<D, FMT, CT, PACKED>(qs, kt, s);
+        if (rb + 1 < row_blocks) raw.load(a, item, hk, (rb + 1) * RB, lane);
+        const int r = rb * RB + (PACKED ? (col & 7) : col);
+        const int lim = r < a.rows && (!PACKED || col < 8) ? row_limit(a, n_kv, r) : 0;
+        float M = 0.f, inv = 0.f;
+        if (lim > k0) {
+            const float2 ml = *reinterpret_cast<const float2 *>(a.row_ml + 2 * row_at(a, item, hk, r));
+            M = ml.x;
+            inv = ml.y != 0.f ? 1.f / ml.y : 0.f;
+        }
 #pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            const int r = rb * RB + (PACKED ? (col & 7) : 16 * t + col);
-            const int lim = r < a.rows && (!PACKED || col < 8) ? row_limit(a, n_kv, r) : 0;
-            float M = 0.f, inv = 0.f;
-            if (lim > k0) {
-                const float *ml = a.row_ml + 2 * row_at(a, item, hk, r);
-                M = ml[0];
-                inv = ml[1] != 0.f ? 1.f / ml[1] : 0.f;
+        for (int n = 0; n < kWeightTiles; ++n) {
+            f32x4 s[CT][kQ];
+            score_tile<D, FMT, CT, PACKED>(qs, kt[n], s);
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) {
+                const float f = qs.back[0] * sk[n].s[q];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = exp2_fast(__builtin_fmaf(s[0][q][i], f, -M)) * inv;
+                    acc[n][q][i] += k0 + n * kTile + 16 * q + 4 * g + i < lim ? p : 0.f;
+                }
             }
-#pragma unroll
-            for (int q = 0; q < kQ; ++q)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (k0 + 16 * q + 4 * g + i < lim)
-                        acc[q][i] += exp2_fast(__builtin_fmaf(s[t][q][i], qs.back[t] * sk.s[q], -M)) * inv;
         }
     }
-    // over the 16 columns
+    // over the 16 columns, all of which then have the sum: column 4 q + i writes key 16 q + 4 g + i
     float *w = a.weights + item * a.w_bstride + hk * a.w_stride;
 #pragma unroll
-    for (int q = 0; q < kQ; ++q)
+    for (int n = 0; n < kWeightTiles; ++n) {
+        float mine = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float x = acc[q][i];
+        for (int q = 0; q < kQ; ++q)
 #pragma unroll
-            for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
-            const int key = k0 + 16 * q + 4 * g + i;
-            // of the columns, all of which have the sum, 4 q + i writes this key
-            if (col == 4 * q + i && key < n_kv) w[key] = (a.decay != 0.f ? a.decay * w[key] : 0.f) + x;
-        }
+            for (int i = 0; i < 4; ++i) {
+                float x = acc[n][q][i];
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
+                if (col == 4 * q + i) mine = x;
+            }
+        const int key = k0 + n * kTile + 16 * (col >> 2) + 4 * g + (col & 3);
+        if (col < 4 * kQ && key < n_kv) w[key] = (a.decay != 0.f ? a.decay * w[key] : 0.f) + mine;
+    }
 }
 
-template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &a, hipStream_t stream) {
+template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &a, bool prompt, hipStream_t stream) {
     constexpr int RB = Geo<D, CT, PACKED>::kRows;
-    const uint64_t blocks = (uint64_t)a.view.n_head_kv * a.row_blocks * a.n_seq * a.max_chunks;
+    const uint64_t blocks = (uint64_t)a.per * a.n_seq * a.max_chunks;
     if (blocks > 0x7fffffffull) return hipErrorInvalidValue;
-    kvq_attn_kernel<D, FMT, CT, PACKED><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(a);
+    if (prompt)
+        kvq_prompt_kernel<D, FMT><<<(unsigned)blocks, 64 * kPromptWaves, 0, stream>>>(a);
+    else
+        kvq_attn_kernel<D, FMT, CT, PACKED><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.max_chunks > 1) {
-        const int64_t rows = (int64_t)a.n_seq * a.view.n_head_kv * a.rows;
-        if (a.max_chunks > kManyChunks)
-            kvq_merge_kernel<D, 16, RB><<<(unsigned)(rows * (D / 16)), 256, 0, stream>>>(a);
-        else
-            kvq_merge_kernel<D, D, RB><<<(unsigned)rows, 256, 0, stream>>>(a);
+        const uint64_t rows = (uint64_t)a.n_seq * a.view.n_head_kv * a.rows;
+        const unsigned few = (unsigned)((rows * (D / 4) + 255) / 256);
+#define ZWG_KVQ_MERGE(RB_)                                                                                         \
+    if (a.max_chunks <= 4)                                                                                        \
+        kvq_merge_few_kernel<D, 4, RB_><<<few, 256, 0, stream>>>(a, (int)rows);                                   \
+    else if (a.max_chunks <= 8)                                                                                   \
+        kvq_merge_few_kernel<D, 8, RB_><<<few, 256, 0, stream>>>(a, (int)rows);                                   \
+    else if (a.max_chunks <= 16)                                                                                  \
+        kvq_merge_few_kernel<D, 16, RB_><<<few, 256, 0, stream>>>(a, (int)rows);                                  \
+    else if (a.max_chunks <= kManyChunks)                                                                         \
+        kvq_merge_kernel<D, D, RB_><<<(unsigned)rows, 256, 0, stream>>>(a);                                       \
+    else                                                                                                          \
+        kvq_merge_kernel<D, 16, RB_><<<(unsigned)(rows * (D / 16)), 256, 0, stream>>>(a);
+        if (prompt) {
+            ZWG_KVQ_MERGE(kPromptRows)
+        } else {
+            ZWG_KVQ_MERGE(RB)
+        }
+#undef ZWG_KVQ_MERGE
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.weights && a.n_kv > 0) {
-        const dim3 grid((unsigned)(a.view.n_head_kv * a.n_seq), (unsigned)((a.n_kv + kTile - 1) / kTile));
-        kvq_weights_kernel<D, FMT, CT, PACKED><<<grid, 64, 0, stream>>>(a);
+        const dim3 grid((unsigned)(a.view.n_head_kv * a.n_seq), (unsigned)((a.n_kv + kWeightKeys - 1) / kWeightKeys));
+        kvq_weights_kernel<D, FMT, PACKED><<<grid, 64, 0, stream>>>(a);
         e = hipGetLastError();
     }
     return e;
 }
 
-template <int D, int FMT> hipError_t launch_rows(const KvqArgs &a, hipStream_t stream) {
-    return a.rows <= kKvqPackedRows ? launch<D, FMT, 1, true>(a, stream) : launch<D, FMT, 2, false>(a, stream);
+template <int D, int FMT> hipError_t launch_rows(const KvqArgs &a, bool prompt, hipStream_t stream) {
+    return a.rows <= kKvqPackedRows ? launch<D, FMT, 1, true>(a, false, stream) : launch<D, FMT, 2, false>(a, prompt, stream);
 }
 
 int attention(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const float *q, const zwg_kvq_attn &s,
@@ -741,9 +978,10 @@ int attention(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const 
     hipError_t e = hipSetDevice(ctx->device);
     if (e != hipSuccess) return fail_hip(ctx, "hipSetDevice", e);
 
-    const uint64_t RB = rows <= kKvqPackedRows ? 8 : 32;
+    const bool prompt = rows > kKvqPackedRows && kvq_prompt(rows, n_seq * d.n_head_kv, s.n_kv);
+    const uint64_t RB = rows <= kKvqPackedRows ? 8 : prompt ? kPromptRows : 32;
     const uint64_t n_rows = n_seq * d.n_head_kv * rows, row_blocks = (rows + RB - 1) / RB;
-    const KvqSplit sp = kvq_split(n_seq * d.n_head_kv * row_blocks, s.n_kv, n_rows, d.d, weights != nullptr, ctx->workspace_bytes);
+    const KvqSplit sp = kvq_split(n_seq * d.n_head_kv * row_blocks, s.n_kv, n_rows, d.d, weights != nullptr, ctx->workspace_bytes, prompt);
     const KvqWorkspace ws = kvq_workspace(n_rows, (uint64_t)sp.max_chunks, d.d, weights != nullptr);
     if (ws.total * sizeof(float) > ctx->workspace_bytes)
         return fail(ctx, "the context's workspace is smaller than the rows' statistics (weights)");
@@ -785,9 +1023,9 @@ int attention(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const 
     a.w_bstride = (int64_t)s.weights_bstride;
     a.decay = s.decay;
     switch (d.d) {
-    case 32: e = d.format == ZWG_KVQ_I8 ? launch_rows<32, 0>(a, ctx->stream) : launch_rows<32, 1>(a, ctx->stream); break;
-    case 64: e = d.format == ZWG_KVQ_I8 ? launch_rows<64, 0>(a, ctx->stream) : launch_rows<64, 1>(a, ctx->stream); break;
-    default: e = d.format == ZWG_KVQ_I8 ? launch_rows<128, 0>(a, ctx->stream) : launch_rows<128, 1>(a, ctx->stream); break;
+    case 32: e = d.format == ZWG_KVQ_I8 ? launch_rows<32, 0>(a, prompt, ctx->stream) : launch_rows<32, 1>(a, prompt, ctx->stream); break;
+    case 64: e = d.format == ZWG_KVQ_I8 ? launch_rows<64, 0>(a, prompt, ctx->stream) : launch_rows<64, 1>(a, prompt, ctx->stream); break;
+    default: e = d.format == ZWG_KVQ_I8 ? launch_rows<128, 0>(a, prompt, ctx->stream) : launch_rows<128, 1>(a, prompt, ctx->stream); break;
     }
     return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "kvq attention launch", e);
 }

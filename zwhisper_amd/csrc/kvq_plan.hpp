@@ -233,6 +233,15 @@ inline uint64_t kvq_cut_bytes(uint64_t units, const zwg_kvq_cut &c) {
 constexpr int kKvqWaves = 4; // waves of a workgroup, over the keys
 constexpr int kKvqSplitTile = zwg::kKvqTile * kKvqWaves;
 constexpr int kKvqPackedRows = 8;
+// Which calls of more than 8 rows (queries x heads of a KV head) take the prompt kernel (128 rows to a workgroup that share
+// operands in LDS) and not the one that splits the keys over a workgroup's waves (32 rows): those with rows for most of a
+// workgroup and enough products to fill the card with such workgroups, fewer where the keys are many.  Measured, split keys
+// against prompt, us a call, d = 128, two KV heads: 6144 rows x 8000 keys 186 : 123, 2400 x 4000 41.7 : 42.3, 1152 x 4000
+// 29.7 : 32.8, 576 x 4000 21.3 : 30.3, 192 x 30,000 64.9 : 48.1, 144 x 30,000 54.9 : 48.2, 96 x 30,000 38.4 : 44.9.
+inline bool kvq_prompt(uint64_t rows, uint64_t units, uint64_t n_kv) {
+    const uint64_t pairs = rows * units * n_kv; // below 2^31 * 2^31
+    return rows >= 112 && pairs >= (n_kv >= 16384 ? 1ull << 23 : 1ull << 24);
+}
 constexpr uint64_t kKvqMaxChunks = 4096;
 
 inline std::string check_kvq_attn(const zwg_kvq_desc &d, uint64_t layer, uint64_t seq0, uint64_t n_seq, const float *q,
@@ -260,7 +269,7 @@ inline std::string check_kvq_attn(const zwg_kvq_desc &d, uint64_t layer, uint64_
         if (d.n_head_kv > 1 && s.weights_stride < s.n_kv) return "weights_stride is smaller than n_kv";
         if (n_seq > 1 && s.weights_bstride < (d.n_head_kv - 1) * s.weights_stride + s.n_kv)
             return "weights_bstride is smaller than a sequence's weights";
-        if ((s.n_kv + zwg::kKvqTile - 1) / zwg::kKvqTile > 65535) return "weights: n_kv must be below 2^21";
+        if (s.n_kv > 65535ull * 128) return "weights: n_kv must be below 65535 * 128";
     }
     if (s.n_q * s.n_head * n_seq > 0x7fffffffull) return "n_q * n_head * sequences must be below 2^31";
     return "";
@@ -292,7 +301,11 @@ struct KvqSplit {
 constexpr uint64_t kKvqLongChunk = 4;
 constexpr uint64_t kKvqUnsplit = 6;
 
-inline KvqSplit kvq_split(uint64_t units, uint64_t n_kv, uint64_t rows, uint64_t d, bool weights, uint64_t ws_bytes) {
+//
+// Prompts (workgroups of 128 rows, two to a CU, a tile of 128 keys 5.8 us when both are there, about a tile more at a
+// workgroup's ends): the chunk count of the least time over whole rounds of 512 workgroups and the merge, which reads
+// the partials at 3.3 TB/s.  Measured, 1024 queries over 8000 keys (96 units): 10 chunks 126 + 20 us, 5 chunks 124 + 11.
+inline KvqSplit kvq_split(uint64_t units, uint64_t n_kv, uint64_t rows, uint64_t d, bool weights, uint64_t ws_bytes, bool prompt) {
     const uint64_t w = std::max<uint64_t>(1, (n_kv + kKvqSplitTile - 1) / kKvqSplitTile);
     const auto tiles = [&](uint64_t blocks) {
         const uint64_t want = std::min<uint64_t>(w, std::max<uint64_t>(1, (blocks + units - 1) / units));
@@ -300,7 +313,17 @@ inline KvqSplit kvq_split(uint64_t units, uint64_t n_kv, uint64_t rows, uint64_t
     };
     uint64_t tau = tiles(512);
     if (tau > kKvqLongChunk) tau = std::max(kKvqLongChunk, tiles(1024));
-    if (w <= kKvqUnsplit) tau = w; // up to 6 steps a wave: less than a merge's launch
+    if (prompt) {
+        double best = 0;
+        for (uint64_t c = 1; c <= std::min<uint64_t>(w, 32); ++c) {
+            const double rounds = (double)((units * c + 511) / 512), merge = c > 1 ? (3.0 + (double)(rows * c * d) * 4 / 3.3e6) / 5.8 : 0.0;
+            const double cost = rounds * (double)((w + c - 1) / c + 1) + merge;
+            if (c == 1 || cost < best) {
+                best = cost;
+                tau = (w + c - 1) / c;
+            }
+        }
+    } else if (w <= kKvqUnsplit) tau = w; // up to 6 steps a wave: less than a merge's launch
     const auto bound = [&](uint64_t t) { return std::max<uint64_t>(1, (w + t / 2) / t); };
     while (bound(tau) > 1 && (bound(tau) > kKvqMaxChunks || kvq_workspace(rows, bound(tau), d, weights).total * sizeof(float) > ws_bytes))
         ++tau;
