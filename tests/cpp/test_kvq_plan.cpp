@@ -224,7 +224,42 @@ static void splits() {
     }
 }
 
+// An eviction's groups cover the kept tokens; its lists, flags and ticket are counted; its grid stays in range.
+static void cuts() {
+    std::mt19937_64 rng(6);
+    for (int it = 0; it < 20000; ++it) {
+        const zwg_kvq_desc d{1, 1, 1 << 24, 1, 32u << (rng() % 3), 16u << (rng() % 3), ZWG_KVQ_I8, 0};
+        const uint64_t units = 1 + rng() % 300;
+        zwg_kvq_cut c{};
+        c.n_kv = rng() % (it % 2 ? 5000 : 1 << 24);
+        c.n_keep = 1 + rng() % (c.n_kv + 10);
+        const KvqCutPlan p = kvq_cut_plan(units, d, c);
+        const uint64_t group = kvq_move_group(d.d);
+        if (c.n_keep < c.n_kv) {
+            CHECK(p.groups * group >= c.n_keep && (p.groups - 1) * group < c.n_keep, "groups");
+            CHECK(p.row % 32 == 0 && p.row >= c.n_kv && p.kept % 32 == 0 && p.kept >= units * c.n_keep, "rows");
+            CHECK(p.flags % 32 == 0 && p.flags > p.groups, "flags");
+        } else {
+            CHECK(p.groups == 1 && p.row == 0 && p.kept == 0 && p.flags == 0, "nothing to cut");
+        }
+        CHECK(p.bytes == 4 * (units * (p.row + 2 * p.flags + 1) + p.kept), "bytes");
+    }
+    // 2^21 workgroups at most
+    const float *w = reinterpret_cast<const float *>(256);
+    const uint64_t group = kvq_move_group(128);
+    zwg_kvq_desc d{1u << 21, 1, 4096, 1, 128, 16, ZWG_KVQ_I8, 0};
+    zwg_kvq_cut c{};
+    c.n_kv = 4096;
+    c.n_keep = group;
+    c.weights_stride = 4096;
+    CHECK(check_kvq_cut(d, 0, 1u << 20, 0, 1, c, w, nullptr).empty(), "in range");
+    CHECK(!check_kvq_cut(d, 0, (1u << 20) + 1, 0, 1, c, w, nullptr).empty(), "out of range");
+    c.n_keep = group + 1;
+    CHECK(!check_kvq_cut(d, 0, (1u << 19) + 1, 0, 1, c, w, nullptr).empty(), "two groups");
+}
+
 int main() {
+    cuts();
     layout();
     descs();
     calls();

@@ -2,6 +2,8 @@
 to the bit, attention and weights within bounds derived from the arithmetic (_kvq_ref.tolerance)."""
 from __future__ import annotations
 
+import re
+
 import numpy as np
 import pytest
 
@@ -438,6 +440,34 @@ def test_eviction(torch, z, ctx, case, fmt):
                     if step == 0 and m + 3 <= n_ctx:
                         kv.append(layer, s, m, dev(torch, k), dev(torch, v))
                         want[layer, s].append(m, k, v)
+
+
+@pytest.mark.parametrize("d,block,keep", [(32, 16, 4400), (64, 64, 3001), (128, 32, 1300), (128, 16, 2000), (128, 64, 4999)])
+def test_eviction_of_many_groups(torch, z, d, block, keep):
+    """Groups of one unit that move in parallel into each other's old places, with exactly the workspace they need."""
+    H, N = 2, 5000
+    rng = np.random.default_rng(keep)
+    k, v = (rng.standard_normal((N, H, d)).astype(np.float32) for _ in range(2))
+    w = rng.random((1, 1, H, N)).astype(np.float32)
+    with z.Context(0, workspace_bytes=4096) as cx, z.KVQCache(cx, 1, 1, N, H, d, block) as kv:
+        with pytest.raises(z.ZwgError, match="workspace") as e:
+            kv.evict(0, 1, 0, 1, N, keep, dev(torch, w))
+    need = int(re.search(r"needs (\d+) bytes", str(e.value)).group(1))
+    idx = [ref.choose(w[0, 0, h], N, keep, 3, 100) for h in range(H)]
+    c = ref.Cache(N, H, d, block, "i8")
+    c.append(0, k, v)
+    c.evict(idx)
+    with z.Context(0, workspace_bytes=need) as cx, z.KVQCache(cx, 1, 1, N, H, d, block) as kv:
+        for _ in range(3):  # its flags and ticket start over in each call
+            kv.append(0, 0, 0, dev(torch, k), dev(torch, v))
+            kept = torch.empty(1, 1, H, keep, dtype=torch.int32, device="cuda")
+            kv.evict(0, 1, 0, 1, N, keep, dev(torch, w), None, 3, 100, kept=kept)
+            assert kept[0, 0].tolist() == [list(i) for i in idx]
+            for g, x in zip(values(torch, kv, 0, 0, N), c.vals):
+                assert np.array_equal(g, x[:N])
+    with z.Context(0, workspace_bytes=need - 1) as cx, z.KVQCache(cx, 1, 1, N, H, d, block) as kv:
+        with pytest.raises(z.ZwgError, match="workspace"):
+            kv.evict(0, 1, 0, 1, N, keep, dev(torch, w))
 
 
 def test_eviction_without_extras(torch, z, ctx):

@@ -329,6 +329,8 @@ struct CutArgs {
     int32_t *dst;   // [unit of the call][n_kv rounded up to 32]: each token's new position, or -1
     int64_t dst_stride;
     int32_t *count; // [unit of the call]: the tokens before the cut (the counts may be overwritten after it)
+    int32_t *flags; // [unit of the call][keys, values][flag_stride]: a ticket, then for each group: its codes are out of the cache
+    int32_t n_groups, flag_stride;
 };
 
 // A weight as an unsigned number in the order of the selection: negative below positive, the zeros equal, a NaN
@@ -356,6 +358,7 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
     int32_t *src = a.src + cu * a.n_keep, *dst = a.dst + cu * a.dst_stride;
     int32_t *kept = a.kept ? a.kept + cu * a.n_keep : nullptr;
     if (tid == 0) a.count[cu] = n;
+    for (int i = tid; i < 2 * a.flag_stride; i += kSelectThreads) a.flags[2 * cu * a.flag_stride + i] = 0;
     if (n <= a.n_keep) {
         for (int i = tid; i < a.n_keep; i += kSelectThreads)
             if (kept) kept[i] = i < n ? i : -1;
@@ -465,23 +468,44 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
         for (int i = a.n_keep + tid; i < a.n_kv; i += kSelectThreads) w_out[i] = 0.0f;
 }
 
-constexpr int kMoveThreads = 1024;
-constexpr int kMoveWaves = kMoveThreads / 64;
+template <int D> constexpr int kMoveGroup = (int)kvq_move_group(D); // new tokens of a workgroup
+template <int D> constexpr int kMoveThreads = 2 * kMoveGroup<D>;
 
-// One workgroup per (layer, sequence, head) and keys or values: new tokens in groups of kGroup, in ascending order.  A kept
-// token never moves up, so the tokens of a group and of all later ones lie at or above the group's first position: once a
-// group's codes are out of the cache (in registers, or in LDS; what a thread puts into LDS before the barrier depends on its
-// loads) its positions may be overwritten, and no later group misses what was there.
+// Groups of a unit in parallel, in place.  A kept token never moves up, so the old codes under a group's new positions are
+// read by that group and lower ones only: a group takes its own codes out of the cache (into registers, or LDS), says so,
+// and waits for all lower groups of its keys or values to have said so before it writes.  The unit's workgroups take their
+// groups by tickets, in ascending order: what one waits for has a lower ticket and runs already, and the lowest waits for
+// nothing, so every wait ends; the bound on it (seconds) is for a workspace that something else overwrites.  Nothing is
+// passed through the cache from group to group, only the loads' completion, so the flags need no release of the caches.
+//
+// Measured, 112 units of four groups, d = 128: 26 us for 33 MB read and 29 MB written, 2.4 TB/s; with one workgroup taking
+// a unit's groups in turn 34, with the groups gathered into a staging buffer and copied back 32, with one ticket counter for
+// all units 30.6 (its atomics queue up).  What is left is the chain of a group: positions, gather, largest, wait, store.
+constexpr int kMaxPolls = 1 << 22;
+// Behind a barrier: every load of the workgroup from the cache has returned (its value was used before the barrier).
+__device__ __forceinline__ void group_read(const CutArgs &a, int64_t unit2, int group) {
+    if (a.n_groups > 1 && threadIdx.x == 0)
+        __hip_atomic_store(a.flags + unit2 * a.flag_stride + 1 + group, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <int D> __device__ __forceinline__ void await_lower_groups(const CutArgs &a, int64_t unit2, int group) {
+    if (group == 0) return;
+    const int32_t *flags = a.flags + unit2 * a.flag_stride + 1;
+    for (int g = threadIdx.x; g < group; g += kMoveThreads<D>)
+        for (int i = 0; i < kMaxPolls && !__hip_atomic_load(flags + g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); ++i)
+            __builtin_amdgcn_s_sleep(1);
+    __syncthreads();
+}
+
+// New tokens [t0, t0 + kMoveGroup) of a (layer, sequence, head)'s keys or values.
 //
 // Keys: a token's codes are runs of 16 bytes (8 at d = 32), gathered run by run.  Values: a token's codes lie one or two to a
 // 64-byte line, so the old tiles are read whole and in order, each wave one at a time, and their kept tokens' bytes are put into
-// LDS by new position, [d][kGroup].  Both are then taken as words of four codes twice: for the new blocks' largest
-// magnitudes, and for the new codes.
-template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_unit(const CutArgs &a, int64_t cu) {
-    constexpr int kGroup = 65536 / (D < 64 ? 64 : D); // 512 tokens at d = 128, else 1024
+// LDS by new position, [d][group].  Both are taken twice: for the new blocks' largest magnitudes, and for the new codes.
+template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_group(const CutArgs &a, int64_t cu, int group) {
+    constexpr int kGroup = kMoveGroup<D>, kMoveWaves = kMoveThreads<D> / 64;
     constexpr int kRow = kGroup + 16;                 // bytes of a dim's row in LDS: 4 words beyond a multiple of the banks
     constexpr int kRun = D == 32 ? 8 : 16;            // bytes of a key run
-    constexpr int kRuns = kGroup * D / kRun / kMoveThreads; // runs of a thread: 4
+    constexpr int kRuns = kGroup * D / kRun / kMoveThreads<D>; // runs of a thread: 4, at d = 64 and 32 2
     __shared__ uint32_t tops[kGroup / 16];
     __shared__ float scale_s[kGroup];
     __shared__ int32_t src_s[IS_V ? 1 : kGroup];
@@ -493,181 +517,191 @@ template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_unit(co
     const int64_t layer = a.layer0 + cu / ((int64_t)H * a.n_seq);
     const int64_t seq = (cu / H) % a.n_seq, head = cu % H;
     const int n = a.count[cu];
-    if (IS_V && cu < (int64_t)H * a.n_seq && head == 0 && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
+    // the counts may be overwritten now: the kernel before this one read them
+    if (IS_V && group == 0 && cu < (int64_t)H * a.n_seq && head == 0 && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
     if (n <= a.n_keep) return;
     const int64_t u = (layer * v.n_seq + a.seq0 + seq) * H + head;
+    if (group == 0 && tid == 0) v.open[2 * u + IS_V].block = -1; // the open block's rows are others now
+    const int t0 = group * kGroup;
     uint8_t *codes = v.codes[IS_V] + u * v.unit_bytes;
     float *scales = v.scales[IS_V] + u * v.n_blocks;
     const int32_t *src = a.src + cu * a.n_keep;
     const int32_t *dst = a.dst + cu * a.dst_stride;
-    if (tid == 0) v.open[2 * u + IS_V].block = -1; // the open block's rows are others now
     const int end = ((a.n_keep + v.block - 1) >> shift) << shift;
-#pragma unroll 1
-    for (int t0 = 0; t0 < end; t0 += kGroup) {
-        const int live = min(a.n_keep - t0, kGroup); // tokens of the group; the rest up to `end` becomes zeros
-        if (tid < kGroup / 16) tops[tid] = 0;
-        for (int t = tid; t < kGroup; t += kMoveThreads) {
-            const int p = t < live ? src[t0 + t] : 0;
-            scale_s[t] = t < live ? scales[p >> shift] : 0.f;
-            if (!IS_V) src_s[t] = p;
-        }
-        u32x4 run[IS_V ? 1 : kRuns];
-        if (!IS_V) {
-            __syncthreads();
+    const int live = min(a.n_keep - t0, kGroup); // tokens of the group; the rest up to `end` becomes zeros
+    if (tid < kGroup / 16) tops[tid] = 0; // fewer than threads
+    for (int t = tid; t < kGroup; t += kMoveThreads<D>) {
+        const int p = t < live ? src[t0 + t] : 0;
+        scale_s[t] = t < live ? scales[p >> shift] : 0.f;
+        if (!IS_V) src_s[t] = p;
+    }
+    u32x4 run[IS_V ? 1 : kRuns];
+    if (!IS_V) {
+        __syncthreads();
 #pragma unroll
-            for (int k = 0; k < kRuns; ++k) {
-                const int w = k * kMoveThreads + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
-                run[k] = (u32x4){0u, 0u, 0u, 0u};
-                if (t < live) {
-                    const uint8_t *at = codes + zwg::kvq_at(0, src_s[t], c, D);
-                    if (kRun == 16) {
-                        run[k] = *reinterpret_cast<const u32x4 *>(at);
-                    } else {
-                        const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
-                        run[k] = (u32x4){x[0], x[1], 0u, 0u};
-                    }
-                }
-            }
-            // a wave's 64 runs are of at most 16 aligned tokens: of one block
-#pragma unroll
-            for (int k = 0; k < kRuns; ++k) {
-                const int t = (k * kMoveThreads + tid) / (D / kRun);
-                // the largest code's value is the largest (one factor for all, and rounding keeps the order)
-                float m = 0.f;
-#pragma unroll
-                for (int i = 0; i < kRun; ++i) m = fmaxf(m, fabsf(code_of<FMT>(run[k], i)));
-                uint32_t top = t < live ? abs_bits(m * scale_s[t]) : 0u;
-#pragma unroll
-                for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
-                if (lane == 0) atomicMax(&tops[t >> shift], top);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kRuns; ++k) {
-                const int w = k * kMoveThreads + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
-                if (t0 + t >= end) continue;
-                float scale, mul;
-                zwg::kvq_scale<FMT>(tops[t >> shift], &scale, &mul);
-                const float s = scale_s[t];
-                uint32_t word[kRun / 4];
-#pragma unroll
-                for (int i = 0; i < kRun / 4; ++i) {
-                    const bool on = t < live;
-                    word[i] = zwg::kvq_encode4<FMT>(on ? code_of<FMT>(run[k], 4 * i) * s : 0.f, on ? code_of<FMT>(run[k], 4 * i + 1) * s : 0.f,
-                                                    on ? code_of<FMT>(run[k], 4 * i + 2) * s : 0.f,
-                                                    on ? code_of<FMT>(run[k], 4 * i + 3) * s : 0.f, mul);
-                }
-                uint8_t *at = codes + zwg::kvq_at(0, t0 + t, c, D);
-                if (kRun == 16)
-                    *reinterpret_cast<u32x4 *>(at) = (u32x4){word[0], word[1], word[kRun / 4 - 2], word[kRun / 4 - 1]};
-                else
-                    *reinterpret_cast<u32x2 *>(at) = (u32x2){word[0], word[1]};
-                if (c == 0 && ((t0 + t) & (v.block - 1)) == 0) scales[(t0 + t) >> shift] = scale;
-            }
-        } else {
-            // the old tiles that hold the group's tokens
-            const int first = src[t0] >> 5, last = src[t0 + live - 1] >> 5;
-            const int g = lane >> 4, col = lane & 15;
-            for (int tile = first + wave; tile <= last; tile += kMoveWaves) {
-                int32_t to[8];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int4 x = *reinterpret_cast<const int4 *>(dst + 32 * tile + 16 * q + 4 * g);
-                    to[4 * q] = x.x - t0;
-                    to[4 * q + 1] = x.y - t0;
-                    to[4 * q + 2] = x.z - t0;
-                    to[4 * q + 3] = x.w - t0;
-                }
-                u32x4 w[D / 32];
-#pragma unroll
-                for (int k = 0; k < D / 32; ++k)
-                    w[k] = *reinterpret_cast<const u32x4 *>(codes + (int64_t)tile * 32 * D + 1024 * k + 64 * col + 16 * g);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (to[e] >= 0 && to[e] < live) // -1, a token of another group: not here
-#pragma unroll
-                        for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                vals[(32 * k + 16 * h + col) * kRow + to[e]] = (uint8_t)(w[k][2 * h + (e >> 2)] >> (8 * (e & 3)));
-            }
-            __syncthreads();
-            // new tiles, a wave to 32 tokens: lane (g, col) takes the 16 bytes of each KB that it would read there, from rows 4
-            // words (mod 64) apart at words g apart: all banks.  Word 2 h + q: dim 32 i + 16 h + col of tokens 16 q + 4 g ..
-            constexpr int kTiles = kGroup / 32 / kMoveWaves; // of a wave: 1 at d = 128, else 2
-            constexpr int kN = D / 32;
-            u32x4 code[kTiles][kN];
-#pragma unroll
-            for (int k = 0; k < kTiles; ++k) {
-                const int t = 32 * (k * kMoveWaves + wave);
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int tq = t + 16 * q + 4 * g;
-                    float m[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < kN; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            code[k][i][2 * h + q] = *reinterpret_cast<const uint32_t *>(&vals[(32 * i + 16 * h + col) * kRow + tq]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(code_of<FMT>(code[k][i], 4 * (2 * h + q) + e)));
-                        }
-                    const float4 s = *reinterpret_cast<const float4 *>(&scale_s[tq]);
-                    uint32_t top = tq < live ? abs_bits(m[0] * s.x) : 0u;
-                    top = max(top, tq + 1 < live ? abs_bits(m[1] * s.y) : 0u);
-                    top = max(top, tq + 2 < live ? abs_bits(m[2] * s.z) : 0u);
-                    top = max(top, tq + 3 < live ? abs_bits(m[3] * s.w) : 0u);
-#pragma unroll
-                    for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
-                    if (lane == 0) atomicMax(&tops[(t + 16 * q) >> shift], top);
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kTiles; ++k) {
-                const int t = 32 * (k * kMoveWaves + wave);
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int tq = t + 16 * q + 4 * g;
-                    float scale, mul;
-                    zwg::kvq_scale<FMT>(tops[(t + 16 * q) >> shift], &scale, &mul);
-                    if (lane == 0 && ((t + 16 * q) & (v.block - 1)) == 0 && t0 + t + 16 * q < end)
-                        scales[(t0 + t + 16 * q) >> shift] = scale;
-                    const float4 s4 = *reinterpret_cast<const float4 *>(&scale_s[tq]);
-                    const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                    for (int i = 0; i < kN; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float x[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                x[e] = tq + e < live ? code_of<FMT>(code[k][i], 4 * (2 * h + q) + e) * s[e] : 0.f;
-                            code[k][i][2 * h + q] = zwg::kvq_encode4<FMT>(x[0], x[1], x[2], x[3], mul);
-                        }
-                }
-#pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    // a last block of 16 may end in the middle of a tile: what lies behind it stays
-                    uint8_t *to = codes + (int64_t)(t0 + t) * D + 1024 * i + 64 * col + 16 * g;
-                    if (t0 + t + 16 < end) {
-                        *reinterpret_cast<u32x4 *>(to) = code[k][i];
-                    } else if (t0 + t < end) {
-                        *reinterpret_cast<uint32_t *>(to) = code[k][i][0];
-                        *reinterpret_cast<uint32_t *>(to + 8) = code[k][i][2];
-                    }
+        for (int k = 0; k < kRuns; ++k) {
+            const int w = k * kMoveThreads<D> + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
+            run[k] = (u32x4){0u, 0u, 0u, 0u};
+            if (t < live) {
+                const uint8_t *at = codes + zwg::kvq_at(0, src_s[t], c, D);
+                if (kRun == 16) {
+                    run[k] = *reinterpret_cast<const u32x4 *>(at);
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                    run[k] = (u32x4){x[0], x[1], 0u, 0u};
                 }
             }
         }
-        __syncthreads(); // the group's LDS is free, its codes written
+        // a wave's 64 runs are of at most 16 aligned tokens: of one block
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+            const int t = (k * kMoveThreads<D> + tid) / (D / kRun);
+            // the largest code's value is the largest (one factor for all, and rounding keeps the order)
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) m = fmaxf(m, fabsf(code_of<FMT>(run[k], i)));
+            uint32_t top = t < live ? abs_bits(m * scale_s[t]) : 0u;
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+            if (lane == 0) atomicMax(&tops[t >> shift], top);
+        }
+        __syncthreads();
+        group_read(a, 2 * cu + IS_V, group);
+        float scale[kRuns];
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+            const int t = (k * kMoveThreads<D> + tid) / (D / kRun);
+            float mul;
+            zwg::kvq_scale<FMT>(tops[t >> shift], &scale[k], &mul);
+            const float s = scale_s[t];
+#pragma unroll
+            for (int i = 0; i < kRun / 4; ++i) {
+                const bool on = t < live;
+                run[k][i] = zwg::kvq_encode4<FMT>(on ? code_of<FMT>(run[k], 4 * i) * s : 0.f, on ? code_of<FMT>(run[k], 4 * i + 1) * s : 0.f,
+                                                  on ? code_of<FMT>(run[k], 4 * i + 2) * s : 0.f,
+                                                  on ? code_of<FMT>(run[k], 4 * i + 3) * s : 0.f, mul);
+            }
+        }
+        await_lower_groups<D>(a, 2 * cu + IS_V, group);
+#pragma unroll
+        for (int k = 0; k < kRuns; ++k) {
+            const int w = k * kMoveThreads<D> + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
+            if (t0 + t >= end) continue;
+            uint8_t *at = codes + zwg::kvq_at(0, t0 + t, c, D);
+            if (kRun == 16)
+                *reinterpret_cast<u32x4 *>(at) = run[k];
+            else
+                *reinterpret_cast<u32x2 *>(at) = (u32x2){run[k][0], run[k][1]};
+            if (c == 0 && ((t0 + t) & (v.block - 1)) == 0) scales[(t0 + t) >> shift] = scale[k];
+        }
+    } else {
+        // the old tiles that hold the group's tokens
+        const int first = src[t0] >> 5, last = src[t0 + live - 1] >> 5;
+        const int g = lane >> 4, col = lane & 15;
+        for (int tile = first + wave; tile <= last; tile += kMoveWaves) {
+            int32_t to[8];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int4 x = *reinterpret_cast<const int4 *>(dst + 32 * tile + 16 * q + 4 * g);
+                to[4 * q] = x.x - t0;
+                to[4 * q + 1] = x.y - t0;
+                to[4 * q + 2] = x.z - t0;
+                to[4 * q + 3] = x.w - t0;
+            }
+            u32x4 w[D / 32];
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k)
+                w[k] = *reinterpret_cast<const u32x4 *>(codes + (int64_t)tile * 32 * D + 1024 * k + 64 * col + 16 * g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (to[e] >= 0 && to[e] < live) // -1, a token of another group: not here
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            vals[(32 * k + 16 * h + col) * kRow + to[e]] = (uint8_t)(w[k][2 * h + (e >> 2)] >> (8 * (e & 3)));
+        }
+        __syncthreads();
+        group_read(a, 2 * cu + IS_V, group);
+        // new tiles, a wave to 32 tokens: lane (g, col) takes the 16 bytes of each KB that it would read there, from rows 4
+        // words (mod 64) apart at words g apart: all banks.  Word 2 h + q: dim 32 i + 16 h + col of tokens 16 q + 4 g ..
+        static_assert(kGroup == 32 * kMoveWaves);
+        const int t = 32 * wave;
+        constexpr int kN = D / 32;
+        u32x4 code[kN];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int tq = t + 16 * q + 4 * g;
+            float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    code[i][2 * h + q] = *reinterpret_cast<const uint32_t *>(&vals[(32 * i + 16 * h + col) * kRow + tq]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(code_of<FMT>(code[i], 4 * (2 * h + q) + e)));
+                }
+            const float4 s = *reinterpret_cast<const float4 *>(&scale_s[tq]);
+            uint32_t top = tq < live ? abs_bits(m[0] * s.x) : 0u;
+            top = max(top, tq + 1 < live ? abs_bits(m[1] * s.y) : 0u);
+            top = max(top, tq + 2 < live ? abs_bits(m[2] * s.z) : 0u);
+            top = max(top, tq + 3 < live ? abs_bits(m[3] * s.w) : 0u);
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+            if (lane == 0) atomicMax(&tops[(t + 16 * q) >> shift], top);
+        }
+        __syncthreads();
+        float scale[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int tq = t + 16 * q + 4 * g;
+            float mul;
+            zwg::kvq_scale<FMT>(tops[(t + 16 * q) >> shift], &scale[q], &mul);
+            const float4 s4 = *reinterpret_cast<const float4 *>(&scale_s[tq]);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[e] = tq + e < live ? code_of<FMT>(code[i], 4 * (2 * h + q) + e) * s[e] : 0.f;
+                    code[i][2 * h + q] = zwg::kvq_encode4<FMT>(x[0], x[1], x[2], x[3], mul);
+                }
+        }
+        await_lower_groups<D>(a, 2 * cu + IS_V, group);
+        if (lane == 0)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                if (((t + 16 * q) & (v.block - 1)) == 0 && t0 + t + 16 * q < end) scales[(t0 + t + 16 * q) >> shift] = scale[q];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            // a last block of 16 may end in the middle of a tile: what lies behind it stays
+            uint8_t *to = codes + (int64_t)(t0 + t) * D + 1024 * i + 64 * col + 16 * g;
+            if (t0 + t + 16 < end) {
+                *reinterpret_cast<u32x4 *>(to) = code[i];
+            } else if (t0 + t < end) {
+                *reinterpret_cast<uint32_t *>(to) = code[i][0];
+                *reinterpret_cast<uint32_t *>(to + 8) = code[i][2];
+            }
+        }
     }
 }
 
-template <int D, int FMT> __global__ __launch_bounds__(kMoveThreads) void kvq_move_kernel(CutArgs a) {
-    if (blockIdx.x & 1)
-        move_unit<D, FMT, 1>(a, blockIdx.x >> 1);
+template <int D, int FMT> __global__ __launch_bounds__(kMoveThreads<D>) void kvq_move_kernel(CutArgs a) {
+    __shared__ int ticket;
+    const int64_t unit2 = blockIdx.x / (unsigned)a.n_groups;
+    int group = 0;
+    if (a.n_groups > 1) { // else nothing waits
+        if (threadIdx.x == 0) ticket = atomicAdd(a.flags + unit2 * a.flag_stride, 1);
+        __syncthreads();
+        group = ticket;
+    }
+    if (unit2 & 1)
+        move_group<D, FMT, 1>(a, unit2 >> 1, group);
     else
-        move_unit<D, FMT, 0>(a, blockIdx.x >> 1);
+        move_group<D, FMT, 0>(a, unit2 >> 1, group);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -822,11 +856,12 @@ int evict(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_
     const std::string msg = check_kvq_cut(d, layer0, n_layer, seq0, n_seq, *c, weights, weights_out);
     if (!msg.empty()) return fail(ctx, msg);
     if (n_layer == 0 || n_seq == 0) return ZWG_OK;
-    const uint64_t units = n_layer * n_seq * d.n_head_kv, need = kvq_cut_bytes(units, *c);
-    if (need > ctx->workspace_bytes) {
+    const uint64_t units = n_layer * n_seq * d.n_head_kv;
+    const KvqCutPlan plan = kvq_cut_plan(units, d, *c);
+    if (plan.bytes > ctx->workspace_bytes) {
         char buf[200];
-        snprintf(buf, sizeof buf, "this eviction lists %llu bytes of kept positions, more than the context's workspace (%llu): fewer layers or sequences a call",
-                 (unsigned long long)need, (unsigned long long)ctx->workspace_bytes);
+        snprintf(buf, sizeof buf, "this eviction needs %llu bytes of workspace, more than the context's (%llu): fewer layers or sequences a call",
+                 (unsigned long long)plan.bytes, (unsigned long long)ctx->workspace_bytes);
         return fail(ctx, buf);
     }
     hipError_t e = hipSetDevice(ctx->device);
@@ -847,15 +882,18 @@ int evict(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_
     a.kept = c->kept;
     a.w = weights;
     a.w_out = weights_out;
-    a.count = reinterpret_cast<int32_t *>(ctx->workspace);
-    // the new positions in rows of 16-byte multiples, which the kernel reads as such
-    a.dst_stride = (int64_t)kvq_cut_row(*c);
-    a.dst = a.count + (units + 3) / 4 * 4;
-    a.src = a.dst + (c->n_keep < c->n_kv ? units * kvq_cut_row(*c) : 0);
+    a.dst_stride = (int64_t)plan.row;
+    a.n_groups = (int32_t)plan.groups;
+    a.flag_stride = (int32_t)plan.flags;
+    a.dst = reinterpret_cast<int32_t *>(ctx->workspace); // the new positions first: the kernel reads them 16 bytes at a time
+    a.src = a.dst + units * plan.row;
+    a.flags = a.src + plan.kept;
+    a.count = a.flags + 2 * units * plan.flags;
     kvq_select_kernel<<<(unsigned)units, kSelectThreads, 0, ctx->stream>>>(a);
     e = hipGetLastError();
     if (e != hipSuccess) return fail_hip(ctx, "kvq select launch", e);
-    ZWG_KVQ_DISPATCH(kvq_move_kernel, d.d, d.format, <<<(unsigned)(2 * units), kMoveThreads, 0, ctx->stream>>>(a))
+    if (c->n_keep >= c->n_kv && !c->n_kv_out) return ZWG_OK; // nothing goes
+    ZWG_KVQ_DISPATCH(kvq_move_kernel, d.d, d.format, <<<(unsigned)(2 * units * plan.groups), (unsigned)(2 * kvq_move_group(d.d)), 0, ctx->stream>>>(a))
     e = hipGetLastError();
     return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "kvq move launch", e);
 }

@@ -206,6 +206,27 @@ inline std::string check_kvq_rows(const zwg_kvq_desc &d, uint64_t layer0, uint64
     return "";
 }
 
+// New tokens of a workgroup of an eviction: as many codes of d = 128 as two workgroups' LDS hold; a quarter of that many
+// tokens at d = 64 and 32, where more workgroups gain (32 units of 1001 kept tokens: groups of 1024, 512, 256: 16.4, 16.0,
+// 12.1 us; 112 units of 2048 at d = 128, groups of 512, 256: 25.8, 27.8 us).
+constexpr uint64_t kvq_move_group(uint64_t d) { return d == 128 ? 512 : 256; }
+// The workspace of an eviction: each unit's new positions of its tokens (rows of whole tiles), all kept tokens' old ones, a
+// ticket and a flag to each group of its keys, the same of its values (lines of their own, for the tickets' sake), its tokens.
+struct KvqCutPlan {
+    uint64_t row, kept, flags, groups, bytes;
+};
+inline KvqCutPlan kvq_cut_plan(uint64_t units, const zwg_kvq_desc &d, const zwg_kvq_cut &c) {
+    KvqCutPlan p{0, 0, 0, 1, 0};
+    if (c.n_keep < c.n_kv) {
+        p.row = (c.n_kv + 31) / 32 * 32;
+        p.kept = (units * c.n_keep + 31) / 32 * 32;
+        p.groups = (c.n_keep + kvq_move_group(d.d) - 1) / kvq_move_group(d.d);
+        p.flags = (1 + p.groups + 31) / 32 * 32;
+    }
+    p.bytes = 4 * (units * p.row + p.kept + 2 * units * p.flags + units);
+    return p;
+}
+
 inline std::string check_kvq_cut(const zwg_kvq_desc &d, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_t n_seq,
                                  const zwg_kvq_cut &c, const float *weights, const float *weights_out) {
     const std::string msg = check_kvq_range(d, layer0, n_layer, seq0, n_seq);
@@ -218,16 +239,13 @@ inline std::string check_kvq_cut(const zwg_kvq_desc &d, uint64_t layer0, uint64_
     if (off(weights, 3) || off(weights_out, 3) || off(c.kept, 3) || off(c.n_kv_dev, 3) || off(c.n_kv_out, 3))
         return "weights, kept and counts must be 4-byte aligned";
     if (c.weights_stride < c.n_kv || c.weights_stride > kMaxStride) return "weights_stride is smaller than n_kv, or out of range";
-    if (n_layer * n_seq * d.n_head_kv > 0x3fffffffull) return "too many (layer, sequence, head) units in one call";
+    if (c.n_kv > (1ull << 24)) return "n_kv is above 2^24";
+    // the kernels' grids: a launch has fewer than 2^32 threads
+    const uint64_t units = n_layer * n_seq * d.n_head_kv;
+    if (units > (1ull << 21) || 2 * units * kvq_cut_plan(units, d, c).groups > (1ull << 21))
+        return "too many (layer, sequence, head) units of this many tokens in one call";
     return "";
 }
-// The workspace of an eviction, bytes: each unit's tokens, their new positions (rows of whole tiles) and the kept ones' old
-// positions.
-inline uint64_t kvq_cut_row(const zwg_kvq_cut &c) { return (c.n_kv + 31) / 32 * 32; }
-inline uint64_t kvq_cut_bytes(uint64_t units, const zwg_kvq_cut &c) {
-    return ((units + 3) / 4 * 4 + (c.n_keep < c.n_kv ? units * (c.n_keep + kvq_cut_row(c)) : 0)) * sizeof(int32_t);
-}
-
 // ---- attention over them
 
 constexpr int kKvqWaves = 4; // waves of a workgroup, over the keys
