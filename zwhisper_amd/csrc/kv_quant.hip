@@ -341,13 +341,16 @@ __device__ __forceinline__ uint32_t rank_bits(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One workgroup per (layer, sequence, head): the threshold weight by four passes over 8 bits each (counts in
-// LDS, whole numbers, so their order does not matter), then one ordered pass that writes the kept positions
-// and weights.  Equal weights at the threshold go to the lowest positions.
+// One workgroup per (layer, sequence, head): the threshold weight by four passes over 8 bits each (counts in LDS, whole
+// numbers, so their order does not matter), then an ordered pass that writes the kept positions and weights.  Equal weights
+// at the threshold go to the lowest positions.  Of 8192 weights each thread holds 8 in registers over all passes; what is
+// left is launch, loads and barriers (measured: 56 units of 2304 weights 10.8 us, 32 of 4096 12.0; with two barriers to each 1024 weights 10.9 and 13.3).
+constexpr int kHeld = 8;
 __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
-    __shared__ uint32_t hist[256];
+    __shared__ uint32_t hist[2][256];
     __shared__ uint32_t found_prefix, found_left;
-    __shared__ int wave_more[kSelectWaves], wave_ties[kSelectWaves];
+    __shared__ uint2 counts[kHeld][kSelectWaves]; // weights above the threshold, and at it: first a wave's, then those before it
+    __shared__ uint2 all;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t cu = blockIdx.x; // unit of the call
     const int H = a.view.n_head_kv;
@@ -367,33 +370,34 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
         return;
     }
     const int lo = a.n_first, hi = n - a.n_recent; // the contested positions
-    // the first 8 of a thread's ranks stay in registers over the passes
-    constexpr int kHeld = 8;
-    uint32_t held[kHeld];
+    constexpr int kSpan = kHeld * kSelectThreads;
+    float held[kHeld]; // of positions base + tid + kSelectThreads k
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
-        const int i = lo + tid + k * kSelectThreads;
-        held[k] = i < hi ? rank_bits(w[i]) : 0u;
+        const int i = tid + k * kSelectThreads;
+        held[k] = i < n ? w[i] : 0.0f;
     }
+    if (tid < 256) hist[0][tid] = 0;
+    __syncthreads();
     uint32_t prefix = 0, left = (uint32_t)(a.n_keep - a.n_first - a.n_recent); // < hi - lo
 #pragma unroll 1
     for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const auto count = [&](uint32_t r) {
-            if (shift == 24 || (r >> (shift + 8)) == prefix) atomicAdd(&hist[(r >> shift) & 255u], 1u);
+        uint32_t *h = hist[(shift >> 3) & 1 ? 0 : 1];
+        const auto count = [&](int i, float x) {
+            const uint32_t r = rank_bits(x);
+            if (i >= lo && i < hi && (shift == 24 || (r >> (shift + 8)) == prefix)) atomicAdd(&h[(r >> shift) & 255u], 1u);
         };
 #pragma unroll
         for (int k = 0; k < kHeld; ++k)
-            if (lo + tid + k * kSelectThreads < hi) count(held[k]);
-        for (int i = lo + tid + kHeld * kSelectThreads; i < hi; i += kSelectThreads) count(rank_bits(w[i]));
+            if (k * kSelectThreads < n) count(tid + k * kSelectThreads, held[k]);
+        for (int i = kSpan + tid; i < hi; i += kSelectThreads) count(i, w[i]);
         __syncthreads();
         if (wave == 0) {
             // the digit at which the counts from the top reach `left`: four digits a lane, lane 0 the highest
             uint32_t c[4], s = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                c[k] = hist[255 - 4 * lane - k];
+                c[k] = h[255 - 4 * lane - k];
                 s += c[k];
             }
             uint32_t incl = s;
@@ -413,56 +417,74 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
                     before += c[k];
                 }
             }
+        } else if (tid >= 256 && tid < 512) {
+            hist[(shift >> 3) & 1][tid - 256] = 0; // the next pass's
         }
         __syncthreads();
         prefix = found_prefix;
         left = found_left;
-        __syncthreads();
     }
     // now `prefix` is the threshold and `left` of its equals stay (none contested: nothing stays between)
     const bool any = a.n_keep > a.n_first + a.n_recent;
-    int done = 0, ties = 0; // kept so far, and ties met so far
-    for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-        const int i = i0 + tid;
-        float wi = 0.0f;
-        bool more = false, tie = false;
-        if (i < n) {
-            wi = w[i];
-            const uint32_t r = rank_bits(wi);
-            const bool fixed = i < lo || i >= hi;
-            more = fixed || (any && r > prefix);
-            tie = !fixed && any && r == prefix;
+    uint32_t more_before = 0, ties_before = 0; // in the spans so far
+    for (int base = 0; base < n; base += kSpan) {
+        if (base > 0) {
+            __syncthreads(); // the counts are free
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) {
+                const int i = base + tid + k * kSelectThreads;
+                held[k] = i < n ? w[i] : 0.0f;
+            }
         }
-        const unsigned long long tb = __ballot(tie);
-        if (lane == 0) wave_ties[wave] = __popcll(tb);
-        __syncthreads();
-        int t = ties;
-        for (int k = 0; k < kSelectWaves; ++k) {
-            const int c = wave_ties[k];
-            if (k < wave) t += c;
-            ties += c;
-        }
-        t += __popcll(tb & ((1ull << lane) - 1));
-        const bool stays = more || (tie && (uint32_t)t < left);
-        const unsigned long long sb = __ballot(stays);
-        if (lane == 0) wave_more[wave] = __popcll(sb);
-        __syncthreads();
-        int at = done;
-        for (int k = 0; k < kSelectWaves; ++k) {
-            const int c = wave_more[k];
-            if (k < wave) at += c;
-            done += c;
-        }
-        at += __popcll(sb & ((1ull << lane) - 1));
-        // every weight of these positions is read (it decided `stays`, which the barrier above follows), and new
-        // positions never lie above old ones: the weights may be compacted in place
-        if (i < (int)a.dst_stride) dst[i] = stays ? at : -1;
-        if (stays) {
-            src[at] = i;
-            if (kept) kept[at] = i;
-            if (w_out) w_out[at] = wi;
+        const auto is_more = [&](int i, uint32_t r) { return i < n && (i < lo || i >= hi || (any && r > prefix)); };
+        const auto is_tie = [&](int i, uint32_t r) { return i >= lo && i < hi && any && r == prefix; };
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const int i = base + tid + k * kSelectThreads;
+            const uint32_t r = rank_bits(held[k]);
+            const uint2 c = make_uint2((uint32_t)__popcll(__ballot(is_more(i, r))), (uint32_t)__popcll(__ballot(is_tie(i, r))));
+            if (lane == 0) counts[k][wave] = c;
         }
         __syncthreads();
+        if (wave == 0) {
+            // 128 counts in order, two to a lane
+            uint2 *at = &counts[0][0] + 2 * lane;
+            static_assert(kHeld * kSelectWaves == 128);
+            const uint2 c0 = at[0], c1 = at[1];
+            uint32_t x = c0.x + c1.x, y = c0.y + c1.y;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t ox = (uint32_t)__shfl_up((int)x, off), oy = (uint32_t)__shfl_up((int)y, off);
+                if (lane >= off) {
+                    x += ox;
+                    y += oy;
+                }
+            }
+            at[0] = make_uint2(x - c0.x - c1.x, y - c0.y - c1.y);
+            at[1] = make_uint2(x - c1.x, y - c1.y);
+            if (lane == 63) all = make_uint2(x, y);
+        }
+        __syncthreads();
+        // every weight of the span is in registers, and new positions never lie above old ones: the weights may be compacted in place
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const int i = base + tid + k * kSelectThreads;
+            const uint32_t r = rank_bits(held[k]);
+            const bool more = is_more(i, r), tie = is_tie(i, r);
+            const unsigned long long below = (1ull << lane) - 1;
+            const uint2 c = counts[k][wave];
+            const uint32_t ties = ties_before + c.y + __popcll(__ballot(tie) & below);
+            const bool stays = more || (tie && ties < left);
+            const int at = (int)(more_before + c.x + __popcll(__ballot(more) & below) + min(ties, left));
+            if (i < (int)a.dst_stride) dst[i] = stays ? at : -1;
+            if (stays) {
+                src[at] = i;
+                if (kept) kept[at] = i;
+                if (w_out) w_out[at] = held[k];
+            }
+        }
+        more_before += all.x;
+        ties_before += all.y;
     }
     if (w_out)
         for (int i = a.n_keep + tid; i < a.n_kv; i += kSelectThreads) w_out[i] = 0.0f;
@@ -478,7 +500,7 @@ template <int D> constexpr int kMoveThreads = 2 * kMoveGroup<D>;
 // nothing, so every wait ends; the bound on it (seconds) is for a workspace that something else overwrites.  Nothing is
 // passed through the cache from group to group, only the loads' completion, so the flags need no release of the caches.
 //
-// Measured, 112 units of four groups, d = 128: 26 us for 33 MB read and 29 MB written, 2.4 TB/s; with one workgroup taking
+// Measured, 56 units of four groups, d = 128: 26 us for 33 MB read and 29 MB written, 2.4 TB/s; with one workgroup taking
 // a unit's groups in turn 34, with the groups gathered into a staging buffer and copied back 32, with one ticket counter for
 // all units 30.6 (its atomics queue up).  What is left is the chain of a group: positions, gather, largest, wait, store.
 constexpr int kMaxPolls = 1 << 22;

@@ -183,6 +183,7 @@ inline std::string check_kvq_append(const zwg_kvq_desc &d, const zwg_rope_desc *
         if (a.pos > d.n_ctx || a.n > d.n_ctx - a.pos) return "append past the end of the cache (pos + n > n_ctx)";
         if (rope && (a.rope_pos > rope->n_ctx || a.n > rope->n_ctx - a.rope_pos))
             return "rotary positions past the end of the rope (rope_pos + n > its n_ctx)";
+        if (a.n > (1ull << 27)) return "at most 2^27 rows in one call"; // a launch has fewer than 2^32 threads
     }
     if (!a.q && !a.q_out) return "";
     if (!rope) return "q is rotated only when the cache has a rope";
@@ -201,14 +202,14 @@ inline std::string check_kvq_rows(const zwg_kvq_desc &d, uint64_t layer0, uint64
     if (!msg.empty()) return msg;
     if (off(k, 15) || off(v, 15)) return "k_out and v_out must be 16-byte aligned";
     if (off(pos_dev, 3)) return "position arrays must be 4-byte aligned";
-    if (n > 0x7fffffffull || pos0 > 0x7fffffffull) return "positions out of range";
+    if (n > (1ull << 27) || pos0 > 0x7fffffffull) return "positions out of range (at most 2^27 in one call)";
     if (n_layer * n_seq > 65535) return "n_layer * n_seq must be below 65536 in one call";
     return "";
 }
 
 // New tokens of a workgroup of an eviction: as many codes of d = 128 as two workgroups' LDS hold; a quarter of that many
 // tokens at d = 64 and 32, where more workgroups gain (32 units of 1001 kept tokens: groups of 1024, 512, 256: 16.4, 16.0,
-// 12.1 us; 112 units of 2048 at d = 128, groups of 512, 256: 25.8, 27.8 us).
+// 12.1 us; 56 units of 2048 at d = 128, groups of 512, 256: 25.8, 27.8 us).
 constexpr uint64_t kvq_move_group(uint64_t d) { return d == 128 ? 512 : 256; }
 // The workspace of an eviction: each unit's new positions of its tokens (rows of whole tiles), all kept tokens' old ones, a
 // ticket and a flag to each group of its keys, the same of its values (lines of their own, for the tickets' sake), its tokens.
