@@ -427,6 +427,9 @@ int zwg_kvq_rows_dev(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t se
  * h*weights_stride (at least n_kv; floats).  The row's first n_kv elements become decay * old + the sum
  * over the call's queries and over the heads that share the KV head of each key's probability (decay 0: the old
  * values are not read); later elements are left alone.  Sums are taken in a fixed order.
+ *
+ * q, out and weights must not overlap.  Partial results of keys split over workgroups take the context's workspace, as much
+ * of it as there is; weights need 8 bytes of it per query and head.  Asynchronous on the context's stream.
  */
 typedef struct zwg_kvq_attn {
     uint64_t n_q;
@@ -461,10 +464,12 @@ int zwg_kvq_attention_dev(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n
  * at their new positions and zeros from there up to n_kv (the most that any sequence has).  kept (may be NULL):
  * int32 [n_layer][n_seq][n_head_kv][n_keep], the old positions of the kept tokens, -1 past
  * a shorter sequence's end.  n_kv_out (may be n_kv_dev, or NULL): int32[n_seq], min(n_kv, n_keep).
+ * Needs 4 * (n_kv + n_keep + n_keep / 128 + 160) bytes of the context's workspace, at most, per (layer, sequence, head), and
+ * is refused where there is less.  Asynchronous on the context's stream.
  */
 typedef struct zwg_kvq_cut {
-    uint64_t n_kv;            /* tokens, or with n_kv_dev the most that any sequence has; at most n_ctx */
-    uint64_t n_keep;          /* >= 1 */
+    uint64_t n_kv;            /* tokens, or with n_kv_dev the most that any sequence has; at most n_ctx and 2^24 */
+    uint64_t n_keep;          /* 1 .. 2^24 */
     uint64_t n_first;         /* n_first + n_recent <= n_keep */
     uint64_t n_recent;
     uint64_t weights_stride;  /* at least n_kv */

@@ -170,6 +170,8 @@ static void calls() {
     };
     badc([](auto &c) { c.n_kv = 101; }, "n_ctx");
     badc([](auto &c) { c.n_keep = 0; }, "n_keep");
+    badc([](auto &c) { c.n_keep = (1u << 24) + 1; }, "n_keep");
+    badc([](auto &c) { c.n_keep = 0x7fffffff; }, "n_keep");
     badc([](auto &c) { c.n_first = 11; }, "n_first");
     badc([](auto &c) { c.n_first = 2, c.n_recent = kMax; }, "n_first");
     badc([](auto &c) { c.weights_stride = 99; }, "weights_stride");

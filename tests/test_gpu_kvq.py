@@ -684,6 +684,24 @@ def test_refusals(torch, z, ctx):
         z.KVQCache(other, 1, 1, 64, 2, 64, rope=z.Rope(ctx, 16, 64))
 
 
+def test_refusals_of_shared_memory_and_missing_tensors(torch, z, ctx):
+    x = torch.zeros(4, 2, 64, device="cuda")
+    o = torch.zeros_like(x)
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    with z.KVQCache(ctx, 1, 4, 64, 2, 64) as kv:
+        for f, args, kw, msg in [(kv.attention, (0, 0, 4, x, x, 1, 2, 4), {}, "same memory"),
+                                 (kv.attention, (0, 0, 1, x, o, 1, 2, 4), dict(weights=o), "same memory"),
+                                 (kv.attention, (0, 0, 1, x, o, 1, 2, 4), dict(weights=x), "same memory"),
+                                 (kv.append, (0, 0, 0, None, x), {}, "k_rows"), (kv.append, (0, 0, 0, x, None), {}, "null k or v"),
+                                 (kv.append, (0, 0, 2 ** 64, x, x), {}, "whole number"), (kv.append_batch, (0, 0, None, x, x), {}, "pos_dev"),
+                                 (kv.append_batch, (0, 0, [0, 1, 2, 3], x, x), {}, "pos_dev"), (kv.append_batch, (0, 0, i, x, None), {}, "null k or v"),
+                                 (kv.attention, (0, 0, 1, None, o, 1, 2, 4), {}, "null q"),
+                                 (kv.evict, (0, 1, 0, 1, 64, 10, None), {}, "null weights"),
+                                 (kv.evict, (0, 1, 0, 1, 64, 2 ** 31 - 1, x), {}, "n_keep")]:
+            with pytest.raises(z.ZwgError, match=msg):
+                f(*args, **kw)
+
+
 def test_the_context_closes_first(torch, z):
     """Caches and ropes that outlive their context refuse calls; closing them afterwards is safe, in either order."""
     import ctypes

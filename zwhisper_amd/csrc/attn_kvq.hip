@@ -927,7 +927,7 @@ template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq
 template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &a, bool prompt, hipStream_t stream) {
     constexpr int RB = Geo<D, CT, PACKED>::kRows;
     const uint64_t blocks = (uint64_t)a.per * a.n_seq * a.max_chunks;
-    if (blocks > 0x7fffffffull) return hipErrorInvalidValue;
+    if (blocks * 64 * (prompt ? kPromptWaves : kWaves) > 0xffffffffull) return hipErrorInvalidValue; // a launch's threads
     if (prompt)
         kvq_prompt_kernel<D, FMT><<<(unsigned)blocks, 64 * kPromptWaves, 0, stream>>>(a);
     else
@@ -974,6 +974,7 @@ int attention(zwg_kvq *kv, uint64_t layer, uint64_t seq0, uint64_t n_seq, const 
     const std::string msg = check_kvq_attn(d, layer, seq0, n_seq, q, s, out, weights);
     if (!msg.empty()) return fail(ctx, msg);
     if (n_seq == 0 || s.n_q == 0) return ZWG_OK;
+    if (out == q || (weights && (weights == out || weights == q))) return fail(ctx, "q, out and weights must not be the same memory");
     const uint64_t group = s.n_head / d.n_head_kv, rows = s.n_q * group;
     hipError_t e = hipSetDevice(ctx->device);
     if (e != hipSuccess) return fail_hip(ctx, "hipSetDevice", e);

@@ -233,7 +233,7 @@ inline std::string check_kvq_cut(const zwg_kvq_desc &d, uint64_t layer0, uint64_
     const std::string msg = check_kvq_range(d, layer0, n_layer, seq0, n_seq);
     if (!msg.empty()) return msg;
     if (c.n_kv > d.n_ctx) return "n_kv is more than the cache has (n_ctx)";
-    if (c.n_keep == 0 || c.n_keep > 0x7fffffffull) return "n_keep must be at least 1 and below 2^31";
+    if (c.n_keep == 0 || c.n_keep > (1ull << 24)) return "n_keep must be in 1 .. 2^24";
     if (c.n_first > c.n_keep || c.n_recent > c.n_keep - c.n_first) return "n_first + n_recent must be at most n_keep";
     if (n_layer == 0 || n_seq == 0) return "";
     if (!weights && c.n_kv) return "null weights";
@@ -247,6 +247,7 @@ inline std::string check_kvq_cut(const zwg_kvq_desc &d, uint64_t layer0, uint64_
         return "too many (layer, sequence, head) units of this many tokens in one call";
     return "";
 }
+
 // ---- attention over them
 
 constexpr int kKvqWaves = 4; // waves of a workgroup, over the keys

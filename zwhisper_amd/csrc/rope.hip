@@ -131,7 +131,9 @@ int apply(zwg_rope *rope, const float *x, uint64_t n, uint64_t n_head, uint64_t 
     a.pieces = in_place ? zwg::rope_turned(a.view) : zwg::rope_pieces(a.view);
     const uint64_t per = n_head * (uint64_t)a.pieces; // at most 65535 * 1024
     a.tokens = (int32_t)std::max<uint64_t>(1, std::min<uint64_t>(n, 4 * kRopeThreads / per));
-    rope_kernel<<<(unsigned)((n + a.tokens - 1) / a.tokens), kRopeThreads, 0, ctx->stream>>>(a);
+    const uint64_t blocks = (n + a.tokens - 1) / a.tokens;
+    if (blocks * kRopeThreads > 0xffffffffull) return fail(ctx, "too many rows in one call"); // a launch's threads
+    rope_kernel<<<(unsigned)blocks, kRopeThreads, 0, ctx->stream>>>(a);
     e = hipGetLastError();
     return e == hipSuccess ? ZWG_OK : fail_hip(ctx, "rope launch", e);
 }

@@ -557,8 +557,8 @@ def _span(n_outer: int, outer: int, n: int, stride: int, row: int) -> int:
 
 def _count(name: str, *values) -> None:
     for v in values:
-        if (v.__class__ is not int and not isinstance(v, (int, np.integer))) or v < 0:
-            raise ZwgError(f"{name} must be a whole number, 0 or more")
+        if (v.__class__ is not int and not isinstance(v, (int, np.integer))) or not 0 <= v < 1 << 63:
+            raise ZwgError(f"{name} must be a whole number, 0 or more (below 2^63)")
 
 
 class Rope(_Handle):
@@ -651,10 +651,11 @@ class KVQCache(_Handle):
         place) rotated at rope_pos.. (None: pos)."""
         rope_pos = pos if rope_pos is None else rope_pos
         _count("layer, seq, pos, rope_pos, n_head and q_stride", layer, seq, pos, rope_pos, n_head, q_stride)
-        n = k_rows.numel() // self.kvw
-        if n * self.kvw != k_rows.numel():
+        kp = self._ptr(k_rows, "k_rows", 0)
+        n = 0 if k_rows is None else k_rows.numel() // self.kvw
+        if k_rows is None or n * self.kvw != k_rows.numel():
             raise ZwgError("k_rows is not whole rows of n_head_kv * d")
-        kp, vp = self._ptr(k_rows, "k_rows", 0), self._ptr(v_rows, "v_rows", n * self.kvw)
+        vp = self._ptr(v_rows, "v_rows", n * self.kvw)
         qp, op, stride = self._queries(q, q_out, n, n_head, q_stride)
         self.ctx._bind_torch_stream()
         self.ctx._check(self._L.zwg_kvq_append(self.handle, layer, seq, pos, n, rope_pos, kp, vp, qp, op, n_head, stride))
@@ -664,8 +665,10 @@ class KVQCache(_Handle):
         """One row per sequence seq0.. at the positions in pos_dev (CUDA int32 tensor), rotated at those of
         rope_pos_dev (None: pos_dev)."""
         _count("layer, seq0, n_head and q_stride", layer, seq0, n_head, q_stride)
-        n = pos_dev.numel()
-        pp, rp = self._ptr(pos_dev, "pos_dev", 0, "int32"), self._ptr(rope_pos_dev, "rope_pos_dev", n, "int32")
+        if pos_dev is None:
+            raise ZwgError("pos_dev must be a CUDA int32 tensor")
+        pp, n = self._ptr(pos_dev, "pos_dev", 0, "int32"), pos_dev.numel()
+        rp = self._ptr(rope_pos_dev, "rope_pos_dev", n, "int32")
         kp, vp = self._ptr(k_rows, "k_rows", n * self.kvw), self._ptr(v_rows, "v_rows", n * self.kvw)
         qp, op, stride = self._queries(q, q_out, n, n_head, q_stride)
         self.ctx._bind_torch_stream()
