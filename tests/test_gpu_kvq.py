@@ -265,6 +265,19 @@ def test_attention(torch, z, ctx, case, fmt):
     kv.close()
 
 
+SPLIT_STEPS = [  # decode steps whose keys are split: up to 16 chunks beside whole and empty sequences, and more than 16
+    ([6000, 1, 0, 900, 300], 1, 12, 2, 128, 32, True), ([5200, 3000], 2, 6, 2, 64, 16, True), ([7000], 4, 2, 1, 32, 32, False),
+    ([12000], 1, 8, 1, 32, 64, True),
+]
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("case", SPLIT_STEPS, ids=lambda c: f"{c[0]}-{c[1:]}".replace(" ", ""))
+def test_weights_of_split_steps(torch, z, ctx, case, fmt):
+    """As test_attention, where the weights form the rows' statistics from those of their chunks, and where they do not."""
+    test_attention(torch, z, ctx, case, fmt)
+
+
 @pytest.mark.parametrize("n_q", [1, 40])
 def test_split_keys_and_small_workspaces(torch, z, ctx, n_q):
     """One long sequence over many chunks, in contexts whose workspaces hold fewer chunks, down to none: within the bounds

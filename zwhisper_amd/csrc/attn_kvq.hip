@@ -158,14 +158,17 @@ template <int FMT> __device__ __forceinline__ f16x8 codes_f16(u32x2 w) {
     return r;
 }
 
+// A register's values moved between the 16 lanes of a row.
+template <int CTRL> __device__ __forceinline__ float dpp_f32(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+
 // x of lane `lane`, the same for the whole wave.
 __device__ __forceinline__ float lane_value(float x, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
 }
 // x of the lane 8 columns away (l ^ 8 within its row of 16).
-__device__ __forceinline__ float other_half(float x) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
-}
+__device__ __forceinline__ float other_half(float x) { return dpp_f32<0x128>(x); } // row_ror 8
 __device__ __forceinline__ float groups_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));
@@ -805,8 +808,7 @@ template <int D, int W, int RB> __global__ __launch_bounds__(256) void kvq_merge
 
 // The same for up to MAXC chunks: a thread per (row, 4 dims), all of its loads on their way at once (those of slots past
 // the row's chunks repeat the last).
-template <int D, int MAXC, int RB> __global__ __launch_bounds__(256) void kvq_merge_few_kernel(KvqArgs a, int n_rows) {
-    const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+template <int D, int MAXC, int RB> __device__ __forceinline__ void merge_few(const KvqArgs &a, int n_rows, int i) {
     const int at = i / (D / 4), c = i % (D / 4);
     if (at >= n_rows) return;
     const int last = a.max_chunks - 1;
@@ -839,6 +841,9 @@ template <int D, int MAXC, int RB> __global__ __launch_bounds__(256) void kvq_me
     }
     store_row<D>(a, item, hk, row, 4 * c, 1, 0, M, L, sum);
 }
+template <int D, int MAXC, int RB> __global__ __launch_bounds__(256) void kvq_merge_few_kernel(KvqArgs a, int n_rows) {
+    merge_few<D, MAXC, RB>(a, n_rows, (int)(blockIdx.x * 256 + threadIdx.x));
+}
 
 // Each key's probability summed over the rows that see it: a wave per 128 keys of a (sequence, KV head) keeps their codes in
 // registers, goes over all row blocks in order, forms the scores again and adds exp2(s - M) / L in its lanes; the columns are
@@ -846,14 +851,16 @@ template <int D, int MAXC, int RB> __global__ __launch_bounds__(256) void kvq_me
 constexpr int kWeightTiles = 4;
 constexpr int kWeightKeys = kWeightTiles * kTile;
 
-template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
+// JOIN: the rows' statistics are not there yet: they are formed from those of their chunks, at most kJoinChunks.
+constexpr int kJoinChunks = 16;
+template <int D, int FMT, bool PACKED, bool JOIN> __device__ __forceinline__ void weigh_keys(const KvqArgs &a, int unit, int piece) {
     constexpr int CT = 1;
     using G = Geo<D, CT, PACKED>;
     constexpr int RB = G::kRows;
     const KvqView &v = a.view;
     const int lane = threadIdx.x, g = lane >> 4, col = lane & 15;
-    const int item = a.by_heads.of((int)blockIdx.x), hk = (int)blockIdx.x - item * v.n_head_kv;
-    const int k0 = blockIdx.y * kWeightKeys;
+    const int item = a.by_heads.of(unit), hk = unit - item * v.n_head_kv;
+    const int k0 = piece * kWeightKeys;
     const int n_kv = item_kv(a, item);
     if (k0 >= n_kv) return;
     const int row_blocks = (a.rows + RB - 1) / RB;
@@ -872,6 +879,14 @@ template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq
         kt[n].load(keys, k < n_kv ? (uint32_t)k * D : kNoStep, lane);
         sk[n].load(v.scales[0] + u * v.n_blocks, k < n_kv ? k : k0, a.block_shift);
     }
+    // the old weights, in the lanes that will write the keys' new ones
+    float *w = a.weights + item * a.w_bstride + hk * a.w_stride;
+    float old[kWeightTiles];
+#pragma unroll
+    for (int n = 0; n < kWeightTiles; ++n) {
+        const int key = k0 + n * kTile + 16 * (col >> 2) + 4 * g + (col & 3);
+        old[n] = a.decay != 0.f && col < 4 * kQ && key < n_kv ? w[key] : 0.f;
+    }
     f32x4 acc[kWeightTiles][kQ];
 #pragma unroll
     for (int n = 0; n < kWeightTiles; ++n)
@@ -879,17 +894,34 @@ template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq
         for (int q = 0; q < kQ; ++q) acc[n][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (; rb < row_blocks; ++rb) {
-        Queries<D, CT, PACKED> qs;
-        qs.take(a, raw, lane);
-        if (rb + 1 < row_blocks) raw.load(a, item, hk, (rb + 1) * RB, lane);
         const int r = rb * RB + (PACKED ? (col & 7) : col);
         const int lim = r < a.rows && (!PACKED || col < 8) ? row_limit(a, n_kv, r) : 0;
         float M = 0.f, inv = 0.f;
         if (lim > k0) {
-            const float2 ml = *reinterpret_cast<const float2 *>(a.row_ml + 2 * row_at(a, item, hk, r));
+            const int64_t at = row_at(a, item, hk, r);
+            float2 ml;
+            int chunk_keys, n_chunks = 1;
+            if (JOIN) n_chunks = split(a, block_limit(a, n_kv, rb, RB), &chunk_keys); // RB: the attention kernel's too
+            if (n_chunks == 1) {
+                ml = *reinterpret_cast<const float2 *>(a.row_ml + 2 * at);
+            } else {
+                const float2 *part = reinterpret_cast<const float2 *>(a.part_ml) + at * a.max_chunks;
+                float2 s[kJoinChunks];
+#pragma unroll
+                for (int k = 0; k < kJoinChunks; ++k) s[k] = part[min(k, n_chunks - 1)];
+                ml = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int k = 0; k < kJoinChunks; ++k) ml.x = fmaxf(ml.x, s[k].x);
+#pragma unroll
+                for (int k = 0; k < kJoinChunks; ++k)
+                    if (k < n_chunks) ml.y += (ml.x == -INFINITY ? 1.f : exp2_fast(s[k].x - ml.x)) * s[k].y;
+            }
             M = ml.x;
             inv = ml.y != 0.f ? 1.f / ml.y : 0.f;
         }
+        Queries<D, CT, PACKED> qs;
+        qs.take(a, raw, lane);
+        if (rb + 1 < row_blocks) raw.load(a, item, hk, (rb + 1) * RB, lane);
 #pragma unroll
         for (int n = 0; n < kWeightTiles; ++n) {
             f32x4 s[CT][kQ];
@@ -905,8 +937,8 @@ template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq
             }
         }
     }
-    // over the 16 columns, all of which then have the sum: column 4 q + i writes key 16 q + 4 g + i
-    float *w = a.weights + item * a.w_bstride + hk * a.w_stride;
+    // over the columns (8 rows: the first 8), all of which then have the sum: column 4 q + i writes key 16 q + 4 g + i
+    static_assert(4 * kQ <= 8);
 #pragma unroll
     for (int n = 0; n < kWeightTiles; ++n) {
         float mine = 0.f;
@@ -915,13 +947,28 @@ template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x = acc[n][q][i];
-#pragma unroll
-                for (int off = 1; off < 16; off <<= 1) x += __shfl_xor(x, off);
+                x += dpp_f32<0xb1>(x);  // quad_perm [1, 0, 3, 2]
+                x += dpp_f32<0x4e>(x);  // quad_perm [2, 3, 0, 1]
+                x += dpp_f32<0x141>(x); // row_half_mirror
+                if (!PACKED) x += dpp_f32<0x140>(x); // row_mirror
                 if (col == 4 * q + i) mine = x;
             }
         const int key = k0 + n * kTile + 16 * (col >> 2) + 4 * g + (col & 3);
-        if (col < 4 * kQ && key < n_kv) w[key] = (a.decay != 0.f ? a.decay * w[key] : 0.f) + mine;
+        if (col < 4 * kQ && key < n_kv) w[key] = (a.decay != 0.f ? a.decay * old[n] : 0.f) + mine;
     }
+}
+
+template <int D, int FMT, bool PACKED> __global__ __launch_bounds__(64) void kvq_weights_kernel(KvqArgs a) {
+    weigh_keys<D, FMT, PACKED, false>(a, blockIdx.x, blockIdx.y);
+}
+// Decode steps: merge and weights in one launch, the merge's workgroups first (merge_y rows of the grid), the weights' with
+// statistics of their own.  One launch less and side by side: 32 sequences of 1 .. 4096 keys (d = 64) 18.9 -> 16.1 us a
+// call.  With more rows the statistics would be joined again by each wave for each row block.
+template <int D, int FMT> __global__ __launch_bounds__(64) void kvq_merge_weights_kernel(KvqArgs a, int n_rows, int merge_y) {
+    if ((int)blockIdx.y < merge_y)
+        merge_few<D, kJoinChunks, kKvqPackedRows>(a, n_rows, (int)((blockIdx.y * gridDim.x + blockIdx.x) * 64 + threadIdx.x));
+    else
+        weigh_keys<D, FMT, true, true>(a, blockIdx.x, (int)blockIdx.y - merge_y);
 }
 
 template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &a, bool prompt, hipStream_t stream) {
@@ -933,8 +980,16 @@ template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &
     else
         kvq_attn_kernel<D, FMT, CT, PACKED><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(a);
     hipError_t e = hipGetLastError();
+    const uint64_t rows = (uint64_t)a.n_seq * a.view.n_head_kv * a.rows;
+    const uint64_t units = (uint64_t)a.view.n_head_kv * a.n_seq, pieces = ((uint64_t)a.n_kv + kWeightKeys - 1) / kWeightKeys;
+    if constexpr (PACKED) {
+        const uint64_t merge_y = (rows * (D / 4) + 64 * units - 1) / (64 * units); // at most 4
+        if (e == hipSuccess && a.weights && a.max_chunks > 1 && a.max_chunks <= kJoinChunks && merge_y + pieces <= 65535) {
+            kvq_merge_weights_kernel<D, FMT><<<dim3((unsigned)units, (unsigned)(merge_y + pieces)), 64, 0, stream>>>(a, (int)rows, (int)merge_y);
+            return hipGetLastError();
+        }
+    }
     if (e == hipSuccess && a.max_chunks > 1) {
-        const uint64_t rows = (uint64_t)a.n_seq * a.view.n_head_kv * a.rows;
         const unsigned few = (unsigned)((rows * (D / 4) + 255) / 256);
 #define ZWG_KVQ_MERGE(RB_)                                                                                         \
     if (a.max_chunks <= 4)                                                                                        \
@@ -956,7 +1011,7 @@ template <int D, int FMT, int CT, bool PACKED> hipError_t launch(const KvqArgs &
         e = hipGetLastError();
     }
     if (e == hipSuccess && a.weights && a.n_kv > 0) {
-        const dim3 grid((unsigned)(a.view.n_head_kv * a.n_seq), (unsigned)((a.n_kv + kWeightKeys - 1) / kWeightKeys));
+        const dim3 grid((unsigned)units, (unsigned)pieces);
         kvq_weights_kernel<D, FMT, PACKED><<<grid, 64, 0, stream>>>(a);
         e = hipGetLastError();
     }
