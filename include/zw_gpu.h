@@ -420,8 +420,8 @@ int zwg_kvq_rows_dev(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t se
  * head h / (n_head / n_head_kv), scores are scaled by f32(1/sqrt(d)), and causal query i sees keys
  * j <= n_kv - n_q + i.  A query that sees no key gives zeros.  The products are f16 MFMA over the codes (exact in
  * f16) and over queries and probabilities split into f16 hi + lo terms, scaled to f16's range row by row, with
- * f32 accumulation: f32-level accuracy for any finite input, measured at most 3e-7 normwise relative beyond what
- * the scores' own f32 rounding gives.
+ * f32 accumulation: f32-level accuracy for any finite input, measured 1.4e-7 to 5.3e-7 normwise relative over up to
+ * 131,001 keys (the same sums in f32 products: 2.2e-7 to 2.1e-6).
  *
  * weights (may be NULL): device f32, sequence i's at weights + i*weights_bstride, KV head h's row at
  * h*weights_stride (at least n_kv; floats).  The row's first n_kv elements become decay * old + the sum
