@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "kv_quant.hpp"
 #include "zw_ctx.hpp"
@@ -66,31 +67,17 @@ __device__ __forceinline__ void write_codes(uint8_t *codes, const float (*rows)[
     }
 }
 
-// One block of a unit: rows [r0, r1) are new (token `tok` on), those before r0 are held in the open block or
-// count as the values of their codes, those from r1 on become zeros.  keep: the block stays open (it is the last
-// that the call touches).
-template <int D, int FMT, int IS_V>
-__device__ void append_block(const AppendArgs &a, int64_t u, int head, int b, int r0, int r1, int64_t tok,
-                             int64_t rope_pos, bool keep, float (*rows)[D + kPad], uint32_t *top, uint32_t *shared_top) {
-    const KvqView &v = a.view;
-    const int B = v.block, tid = threadIdx.x;
-    const int kvw = v.n_head_kv * D;
-    uint8_t *codes = v.codes[IS_V] + u * v.unit_bytes;
-    float *scale_at = v.scales[IS_V] + u * v.n_blocks + b;
-    float *held = v.rows[IS_V] + u * B * D;
-    KvqOpen *open = v.open + 2 * u + IS_V;
-    const int64_t first = (int64_t)b * B;
-
-    const bool is_open = open->block == b;
-    const int filled = is_open ? open->filled : 0;
-    const float old_scale = *scale_at;
-    // the new rows, rotated
+// Rows [r0, r1) of a block, token `tok` on, into LDS, keys rotated, and their largest magnitudes.  Begins and ends without a
+// barrier; what was written to `top` before is there after it for all.
+template <int D, int IS_V>
+__device__ __forceinline__ void new_rows(const AppendArgs &a, int head, int r0, int r1, int64_t tok, int64_t rope_pos,
+                                         float (*rows)[D + kPad], uint32_t *top) {
+    const int tid = threadIdx.x, kvw = a.view.n_head_kv * D;
     for (int i = tid; i < (r1 - r0) * (D / 4); i += kAppendThreads) {
         const int r = i / (D / 4), c = 4 * (i % (D / 4));
         *reinterpret_cast<float4 *>(&rows[r0 + r][c]) =
             *reinterpret_cast<const float4 *>(a.src[IS_V] + (tok + r) * kvw + head * D + c);
     }
-    if (tid < B) top[tid] = tid < r0 && tid < filled ? abs_bits(open->top[tid]) : 0u;
     __syncthreads();
     if (!IS_V && a.rope.cos) {
         const int turned = zwg::rope_turned(a.rope);
@@ -109,6 +96,46 @@ __device__ void append_block(const AppendArgs &a, int64_t u, int head, int b, in
         for (int off = D / 8; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
         if (i % (D / 4) == 0) top[r] = m;
     }
+}
+
+// Rows [from, r1) of block b, and the magnitudes of all before r1, become the unit's open block.
+template <int D, int IS_V>
+__device__ __forceinline__ void hold_rows(const AppendArgs &a, int64_t u, int b, int from, int r1, const float (*rows)[D + kPad],
+                                          const uint32_t *top) {
+    const int tid = threadIdx.x;
+    float *held = a.view.rows[IS_V] + u * a.view.block * D;
+    KvqOpen *open = a.view.open + 2 * u + IS_V;
+    for (int i = tid; i < (r1 - from) * (D / 4); i += kAppendThreads) {
+        const int r = from + i / (D / 4), c = 4 * (i % (D / 4));
+        *reinterpret_cast<float4 *>(held + r * D + c) = *reinterpret_cast<const float4 *>(&rows[r][c]);
+    }
+    if (tid < r1) open->top[tid] = __builtin_bit_cast(float, top[tid]);
+    if (tid == 0) {
+        open->block = b;
+        open->filled = r1;
+    }
+}
+
+// One block of a unit: rows [r0, r1) are new (token `tok` on), those before r0 are held in the open block or
+// count as the values of their codes, those from r1 on become zeros.  keep: the block stays open (it is the last
+// that the call touches, and no other workgroup holds its rows for it).
+template <int D, int FMT, int IS_V>
+__device__ void append_block(const AppendArgs &a, int64_t u, int head, int b, int r0, int r1, int64_t tok,
+                             int64_t rope_pos, bool keep, float (*rows)[D + kPad], uint32_t *top, uint32_t *shared_top) {
+    const KvqView &v = a.view;
+    const int B = v.block, tid = threadIdx.x;
+    uint8_t *codes = v.codes[IS_V] + u * v.unit_bytes;
+    float *scale_at = v.scales[IS_V] + u * v.n_blocks + b;
+    const float *held = v.rows[IS_V] + u * B * D;
+    const KvqOpen *open = v.open + 2 * u + IS_V;
+    const int64_t first = (int64_t)b * B;
+
+    // a block with no rows before the new ones has no use for what is held (which another workgroup may be replacing)
+    const bool is_open = r0 > 0 && open->block == b;
+    const int filled = is_open ? open->filled : 0;
+    const float old_scale = *scale_at;
+    if (tid < B) top[tid] = tid < r0 && tid < filled ? abs_bits(open->top[tid]) : 0u;
+    new_rows<D, IS_V>(a, head, r0, r1, tok, rope_pos, rows, top);
     __syncthreads();
     if (tid < 64) {
         uint32_t m = tid < r1 ? top[tid] : 0u, was = tid < filled ? abs_bits(open->top[tid]) : 0u;
@@ -181,28 +208,17 @@ __device__ void append_block(const AppendArgs &a, int64_t u, int head, int b, in
                 *reinterpret_cast<float4 *>(&rows[from + i / (D / 4)][4 * (i % (D / 4))]) = make_float4(0.f, 0.f, 0.f, 0.f);
             __syncthreads();
         }
-        for (int i = tid; i < (r1 - from) * (D / 4); i += kAppendThreads) {
-            const int r = from + i / (D / 4), c = 4 * (i % (D / 4));
-            *reinterpret_cast<float4 *>(held + r * D + c) = *reinterpret_cast<const float4 *>(&rows[r][c]);
-        }
-        if (tid < r1) open->top[tid] = __builtin_bit_cast(float, top[tid]);
-        if (tid == 0) {
-            open->block = b;
-            open->filled = r1;
-        }
+        hold_rows<D, IS_V>(a, u, b, from, r1, rows, top);
     }
-    __syncthreads(); // the staging may be used for another block
 }
 
 // Workgroups (x, y): y < 2 n_head_kv: head y / 2's keys (y even) or values of the x-th touched block (tokens of one
 // sequence) or of sequence x (one token each); from there on query head y - 2 n_head_kv of the same tokens.
-// The first and the last block of one call both deal with the unit's open block, so one workgroup does them in
-// turn, and a call that touches m blocks has m - 1 of them (at least one).
+// A call's first block b0 may need the unit's open block, which its last one, b1, replaces: where b0 has rows before the new
+// ones, its workgroup also puts b1's rows in their place, after its own use of it, and b1's writes codes alone.
 //
-// Bound by the chain of a block (rows, rotation, largest, codes), not by bytes: 64 sequences' tokens at d = 128 take 6.2 us,
-// 2048 tokens that begin and end inside blocks 11.8, the two blocks of the one workgroup in turn, where the bytes take 4.
-// (A second place for an open block's rows would let the two go side by side, for as many bytes again as short
-// caches have codes.)
+// Bound by the chain of a block (rows, rotation, largest, codes), not by bytes: 64 sequences' tokens at d = 128 take 5.6 us,
+// 2048 that begin and end inside blocks 10.1, and 11.5 with all of b1 behind b0, where the bytes take 4.
 template <int D, int FMT> __global__ __launch_bounds__(kAppendThreads) void kvq_append_kernel(AppendArgs a) {
     __shared__ __align__(16) float rows[zwg::kKvqMaxBlock][D + kPad];
     __shared__ uint32_t top[zwg::kKvqMaxBlock];
@@ -221,33 +237,37 @@ template <int D, int FMT> __global__ __launch_bounds__(kAppendThreads) void kvq_
     }
     const int64_t b0 = pos / B, b1 = (pos + n - 1) / B;
 
+    const int64_t b = b0 + (a.pos_dev ? 0 : x);
+    const int64_t t0 = max(pos, b * B) - pos, t1 = min(pos + n, (b + 1) * B) - pos;
     if (y >= 2 * v.n_head_kv) {
-        // query rows: B tokens a workgroup, as if from the start of the first block
+        // query rows: those of the block's tokens
         const int h = y - 2 * v.n_head_kv;
         const int pieces = a.q == a.q_out ? zwg::rope_turned(a.rope) : zwg::rope_pieces(a.rope);
-        // with one workgroup less than blocks, the first takes the last block's tokens too
-        for (int64_t b = b0 + (a.pos_dev ? 0 : x); b <= b1; b += b1 - b0) {
-            const int64_t t0 = max(pos, b * B) - pos, t1 = min(pos + n, (b + 1) * B) - pos;
-            for (int i = threadIdx.x; i < (int)(t1 - t0) * pieces; i += kAppendThreads) {
-                const int t = i / pieces, c = i - t * pieces;
-                const int64_t row = (tok + t0 + t) * a.q_stride + (int64_t)h * D;
-                zwg::rope_piece(a.rope, rp + t0 + t, c, a.q + row, a.q_out + row);
-            }
-            if (b != b0 || b1 == b0) break;
+        for (int i = threadIdx.x; i < (int)(t1 - t0) * pieces; i += kAppendThreads) {
+            const int t = i / pieces, c = i - t * pieces;
+            const int64_t row = (tok + t0 + t) * a.q_stride + (int64_t)h * D;
+            zwg::rope_piece(a.rope, rp + t0 + t, c, a.q + row, a.q_out + row);
         }
         return;
     }
     const int head = y >> 1;
     u += head;
-    for (int64_t b = b0 + (a.pos_dev ? 0 : x); b <= b1; b += b1 - b0) {
-        const int64_t t0 = max(pos, b * B) - pos, t1 = min(pos + n, (b + 1) * B) - pos;
-        const int r0 = (int)(pos + t0 - b * B), r1 = (int)(pos + t1 - b * B);
-        if (y & 1)
-            append_block<D, FMT, 1>(a, u, head, (int)b, r0, r1, tok + t0, rp + t0, b == b1, rows, top, shared_top);
-        else
-            append_block<D, FMT, 0>(a, u, head, (int)b, r0, r1, tok + t0, rp + t0, b == b1, rows, top, shared_top);
-        if (b != b0 || b1 == b0) break;
-    }
+    const int r0 = (int)(pos + t0 - b * B), r1 = (int)(pos + t1 - b * B);
+    const bool first_holds = b0 < b1 && pos > b0 * B, keep = b == b1 && !first_holds;
+    const int64_t tl = b1 * B - pos; // b1's first token
+    const auto block = [&](auto is_v) {
+        append_block<D, FMT, is_v.value>(a, u, head, (int)b, r0, r1, tok + t0, rp + t0, keep, rows, top, shared_top);
+        if (first_holds && b == b0) {
+            __syncthreads();
+            new_rows<D, is_v.value>(a, head, 0, (int)(n - tl), tok + tl, rp + tl, rows, top);
+            __syncthreads();
+            hold_rows<D, is_v.value>(a, u, (int)b1, 0, (int)(n - tl), rows, top);
+        }
+    };
+    if (y & 1)
+        block(std::integral_constant<int, 1>{});
+    else
+        block(std::integral_constant<int, 0>{});
 }
 
 // ---------------------------------------------------------------------------------------------- reads
@@ -842,7 +862,7 @@ int append(zwg_kvq *kv, const KvqAppend &c, float *q_out) {
     a.rope_pos0 = (int64_t)c.rope_pos;
     a.n = (int32_t)c.n;
     a.n_head = (int32_t)c.n_head;
-    const uint64_t blocks = c.batch ? c.n : std::max<uint64_t>(1, (c.pos + c.n - 1) / d.block - c.pos / d.block);
+    const uint64_t blocks = c.batch ? c.n : (c.pos + c.n - 1) / d.block - c.pos / d.block + 1;
     const dim3 grid((unsigned)blocks, (unsigned)(2 * d.n_head_kv + (c.q ? c.n_head : 0)));
     ZWG_KVQ_DISPATCH(kvq_append_kernel, d.d, d.format, <<<grid, kAppendThreads, 0, ctx->stream>>>(a))
     e = hipGetLastError();
