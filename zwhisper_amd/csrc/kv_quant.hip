@@ -366,14 +366,15 @@ __device__ __forceinline__ uint32_t rank_bits(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One workgroup per (layer, sequence, head): the threshold weight by four passes over 8 bits each (counts in LDS, whole
-// numbers, so their order does not matter), then an ordered pass that writes the kept positions and weights.  Equal weights
+// One workgroup per (layer, sequence, head): the threshold weight by up to four passes over 8 bits each (counts in LDS,
+// whole numbers, so their order does not matter), as many as decide, then an ordered pass that writes the kept positions and weights.  Equal weights
 // at the threshold go to the lowest positions.  Of 8192 weights each thread holds 8 in registers over all passes; what is
-// left is launch, loads and barriers (measured: 56 units of 2304 weights 10.8 us, 32 of 4096 12.0; with two barriers to each 1024 weights 10.9 and 13.3).
+// left is launch, loads and barriers (measured: 56 units of 2304 weights 10.6 us, 32 of 4096 11.3; with two barriers to each
+// 1024 weights 10.9 and 13.3, with 512 threads and 16 weights each 13.4 and 13.7).
 constexpr int kHeld = 8;
 __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
     __shared__ uint32_t hist[2][256];
-    __shared__ uint32_t found_prefix, found_left;
+    __shared__ uint32_t found_prefix, found_left, found_all;
     __shared__ uint2 counts[kHeld][kSelectWaves]; // weights above the threshold, and at it: first a wave's, then those before it
     __shared__ uint2 all;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -404,6 +405,7 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
     }
     if (tid < 256) hist[0][tid] = 0;
     __syncthreads();
+    int low = 0; // bits below the threshold's
     uint32_t prefix = 0, left = (uint32_t)(a.n_keep - a.n_first - a.n_recent); // < hi - lo
 #pragma unroll 1
     for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
@@ -438,6 +440,7 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
                     if (before < left && before + c[k] >= left) {
                         found_prefix = (prefix << 8) | (uint32_t)(255 - 4 * lane - k);
                         found_left = left - before;
+                        found_all = c[k];
                     }
                     before += c[k];
                 }
@@ -448,6 +451,10 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
         __syncthreads();
         prefix = found_prefix;
         left = found_left;
+        if (left == found_all) { // all weights of these digits stay: the lower ones decide nothing
+            low = shift;
+            break;
+        }
     }
     // now `prefix` is the threshold and `left` of its equals stay (none contested: nothing stays between)
     const bool any = a.n_keep > a.n_first + a.n_recent;
@@ -461,8 +468,8 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
                 held[k] = i < n ? w[i] : 0.0f;
             }
         }
-        const auto is_more = [&](int i, uint32_t r) { return i < n && (i < lo || i >= hi || (any && r > prefix)); };
-        const auto is_tie = [&](int i, uint32_t r) { return i >= lo && i < hi && any && r == prefix; };
+        const auto is_more = [&](int i, uint32_t r) { return i < n && (i < lo || i >= hi || (any && (r >> low) > prefix)); };
+        const auto is_tie = [&](int i, uint32_t r) { return i >= lo && i < hi && any && (r >> low) == prefix; };
 #pragma unroll
         for (int k = 0; k < kHeld; ++k) {
             const int i = base + tid + k * kSelectThreads;
