@@ -483,6 +483,51 @@ def test_eviction_of_many_groups(torch, z, d, block, keep):
             kv.evict(0, 1, 0, 1, N, keep, dev(torch, w))
 
 
+def test_evictions_of_many_groups_side_by_side(torch, z):
+    """Two contexts' evictions on streams of their own, eager and as graphs replayed with eager work between: every
+    workgroup that waits for lower groups gets on, and the results are those of one at a time."""
+    H, N, d, keep = 3, 6000, 64, 5001
+    rng = np.random.default_rng(8)
+    k, v = (dev(torch, rng.standard_normal((N, H, d)).astype(np.float32)) for _ in range(2))
+    w = dev(torch, rng.random((2, 1, H, N)).astype(np.float32))
+
+    def step(kv):
+        for layer in range(2):
+            kv.append(layer, 0, 0, k, v)
+        kv.evict(0, 2, 0, 1, N, keep, w, None, 4, 500)
+
+    with z.Context(0) as c0, z.Context(0) as c1, z.Context(0) as c2:
+        with z.KVQCache(c0, 2, 1, N, H, d, 16) as want, z.KVQCache(c1, 2, 1, N, H, d, 16) as a, z.KVQCache(c2, 2, 1, N, H, d, 16) as b:
+            step(want)
+            torch.cuda.synchronize()
+            expected = [values(torch, want, layer, 0, N) for layer in range(2)]
+
+            def check():
+                torch.cuda.synchronize()
+                for kv in (a, b):
+                    for layer in range(2):
+                        for got, x in zip(values(torch, kv, layer, 0, N), expected[layer]):
+                            assert np.array_equal(got, x)
+
+            streams = torch.cuda.Stream(), torch.cuda.Stream()
+            for s, kv in zip(streams, (a, b)):
+                with torch.cuda.stream(s):
+                    for _ in range(3):
+                        step(kv)
+            check()
+            graphs = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+            for g, kv in zip(graphs, (a, b)):
+                with torch.cuda.graph(g):
+                    step(kv)
+            for _ in range(3):
+                for s, g in zip(streams, graphs):
+                    with torch.cuda.stream(s):
+                        g.replay()
+                check()
+                for kv in (a, b):
+                    kv.append(1, 0, 100, k[:77].contiguous(), v[:77].contiguous())
+
+
 def test_eviction_without_extras(torch, z, ctx):
     """No kept list, no new weights, no counts; one count for all; twice (the second cuts nothing); no sequence at all."""
     H, d, N = 2, 64, 90

@@ -343,7 +343,7 @@ constexpr int kSelectWaves = kSelectThreads / 64;
 struct CutArgs {
     KvqView view;
     int64_t layer0, seq0;
-    int32_t n_seq, n_layer;
+    int32_t n_seq;
     int32_t n_kv, n_keep, n_first, n_recent;
     int64_t w_stride;
     const int32_t *n_kv_dev;
@@ -367,7 +367,8 @@ __device__ __forceinline__ uint32_t rank_bits(float w) {
 }
 
 // One workgroup per (layer, sequence, head): the threshold weight by up to four passes over 8 bits each (counts in LDS,
-// whole numbers, so their order does not matter), as many as decide, then an ordered pass that writes the kept positions and weights.  Equal weights
+// whole numbers, so their order does not matter), as many as decide, then an ordered pass that writes the kept positions and
+// weights.  Equal weights
 // at the threshold go to the lowest positions.  Of 8192 weights each thread holds 8 in registers over all passes; what is
 // left is launch, loads and barriers (measured: 56 units of 2304 weights 10.6 us, 32 of 4096 11.3; with two barriers to each
 // 1024 weights 10.9 and 13.3, with 512 threads and 16 weights each 13.4 and 13.7).
@@ -925,7 +926,6 @@ int evict(zwg_kvq *kv, uint64_t layer0, uint64_t n_layer, uint64_t seq0, uint64_
     a.layer0 = (int64_t)layer0;
     a.seq0 = (int64_t)seq0;
     a.n_seq = (int32_t)n_seq;
-    a.n_layer = (int32_t)n_layer;
     a.n_kv = (int32_t)c->n_kv;
     a.n_keep = (int32_t)c->n_keep;
     a.n_first = (int32_t)c->n_first;
