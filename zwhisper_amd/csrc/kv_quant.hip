@@ -370,7 +370,7 @@ __device__ __forceinline__ uint32_t rank_bits(float w) {
 // whole numbers, so their order does not matter), as many as decide, then an ordered pass that writes the kept positions and
 // weights.  Equal weights
 // at the threshold go to the lowest positions.  Of 8192 weights each thread holds 8 in registers over all passes; what is
-// left is launch, loads and barriers (measured: 56 units of 2304 weights 10.6 us, 32 of 4096 11.3; with two barriers to each
+// left is launch, loads and barriers (measured: 56 units of 2304 weights 10.6 us, 32 of 4096 10.9; with two barriers to each
 // 1024 weights 10.9 and 13.3, with 512 threads and 16 weights each 13.4 and 13.7).
 constexpr int kHeld = 8;
 __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
@@ -380,8 +380,7 @@ __global__ __launch_bounds__(kSelectThreads) void kvq_select_kernel(CutArgs a) {
     __shared__ uint2 all;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t cu = blockIdx.x; // unit of the call
-    const int H = a.view.n_head_kv;
-    const int seq = (int)((cu / H) % a.n_seq);
+    const uint32_t seq = blockIdx.x / (uint32_t)a.view.n_head_kv % (uint32_t)a.n_seq;
     const int n = a.n_kv_dev ? min(max(a.n_kv_dev[seq], 0), a.n_kv) : a.n_kv;
     const float *w = a.w + cu * a.w_stride;
     float *w_out = a.w_out ? a.w_out + cu * a.w_stride : nullptr;
@@ -563,19 +562,17 @@ template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_group(c
     constexpr int kRuns = kGroup * D / kRun / kMoveThreads<D>; // runs of a thread: 4, at d = 64 and 32 2
     __shared__ uint32_t tops[kGroup / 16];
     __shared__ float scale_s[kGroup];
-    __shared__ int32_t src_s[IS_V ? 1 : kGroup];
     __shared__ __align__(16) uint8_t vals[IS_V ? D * kRow : 16];
     const KvqView &v = a.view;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int H = v.n_head_kv;
     const int shift = v.block == 16 ? 4 : v.block == 32 ? 5 : 6;
-    const int64_t layer = a.layer0 + cu / ((int64_t)H * a.n_seq);
-    const int64_t seq = (cu / H) % a.n_seq, head = cu % H;
+    const uint32_t H = v.n_head_kv, ls = (uint32_t)cu / H, layer = ls / (uint32_t)a.n_seq; // 32 bits: short divisions
+    const uint32_t seq = ls - layer * a.n_seq, head = (uint32_t)cu - ls * H;
     const int n = a.count[cu];
     // the counts may be overwritten now: the kernel before this one read them
-    if (IS_V && group == 0 && cu < (int64_t)H * a.n_seq && head == 0 && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
+    if (IS_V && group == 0 && layer == 0 && head == 0 && a.n_kv_out && tid == 0) a.n_kv_out[seq] = min(n, a.n_keep);
     if (n <= a.n_keep) return;
-    const int64_t u = (layer * v.n_seq + a.seq0 + seq) * H + head;
+    const int64_t u = ((a.layer0 + layer) * v.n_seq + a.seq0 + seq) * H + head;
     if (group == 0 && tid == 0) v.open[2 * u + IS_V].block = -1; // the open block's rows are others now
     const int t0 = group * kGroup;
     uint8_t *codes = v.codes[IS_V] + u * v.unit_bytes;
@@ -588,17 +585,15 @@ template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_group(c
     for (int t = tid; t < kGroup; t += kMoveThreads<D>) {
         const int p = t < live ? src[t0 + t] : 0;
         scale_s[t] = t < live ? scales[p >> shift] : 0.f;
-        if (!IS_V) src_s[t] = p;
     }
     u32x4 run[IS_V ? 1 : kRuns];
     if (!IS_V) {
-        __syncthreads();
 #pragma unroll
         for (int k = 0; k < kRuns; ++k) {
             const int w = k * kMoveThreads<D> + tid, t = w / (D / kRun), c = kRun * (w % (D / kRun));
             run[k] = (u32x4){0u, 0u, 0u, 0u};
             if (t < live) {
-                const uint8_t *at = codes + zwg::kvq_at(0, src_s[t], c, D);
+                const uint8_t *at = codes + zwg::kvq_at(0, src[t0 + t], c, D);
                 if (kRun == 16) {
                     run[k] = *reinterpret_cast<const u32x4 *>(at);
                 } else {
@@ -607,6 +602,7 @@ template <int D, int FMT, int IS_V> __device__ __forceinline__ void move_group(c
                 }
             }
         }
+        __syncthreads();
         // a wave's 64 runs are of at most 16 aligned tokens: of one block
 #pragma unroll
         for (int k = 0; k < kRuns; ++k) {
